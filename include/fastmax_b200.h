@@ -196,6 +196,94 @@ typedef struct {
 
 int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_decode_args* args, void* cuda_stream);
 
+/* ---- serving: pages of moment states, and trees of drafted tokens ------------------------------------
+ * A page holds one sequence's moment states, heads contiguous: head h of page p at state + p * page_stride + h * rows * ld floats
+ * (rows = fastmax_state_rows, ld = fastmax_state_ld).  A model whose layers share a page passes the layer's first state and the
+ * stride of whole pages.  No counterpart in the reference, which keeps nothing between two calls of its model (transformer/eval.py:8-32). */
+typedef struct {
+  float* state;         /* 16-byte aligned                                                                         */
+  int64_t page_stride;  /* floats; a multiple of 4, at least heads * rows * ld where there is more than one page        */
+  int32_t pages;        /* pages that exist                                                                             */
+  int32_t reserved;
+  const int32_t* table; /* [batch]: the page of each sequence, each page at most once; an entry outside 0 .. pages-1 says that the   */
+                        /* sequence is absent: nothing of it is read or written.  NULL: sequence b has page b (pages >= batch)  */
+} fastmax_pages;
+
+/* fastmax_decode_step with a page per sequence.  The outputs of absent sequences stay as they were. */
+typedef struct {
+  fastmax_tensor q, k, v;
+  fastmax_tensor o;
+  fastmax_tensor g;
+  fastmax_pages cache;
+} fastmax_paged_decode_args;
+int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged_decode_args* args, void* cuda_stream);
+
+/* Attention of a tree of drafted tokens over the cached sequence, which stays as it is:
+ *     o_i = ( sum_r w_r Phi(q_i)_r S[r] + sum_{j in A(i)} f(q_i . k_j * inv_temperature) [v_j | 1] ), divided by its last element,
+ * A(i) = node i and its ancestors; the weights w as in fastmax_decode_step.  One launch, no workspace, the state is read once.
+ *   pb: nq = nk = nodes per sequence, 1 .. FASTMAX_TREE_NODES; `causal` is not used.
+ *   parents (optional): int32 [batch][nq], parents_stride apart: the parent of each node, a node before it, or -1 where the node
+ *       follows the cached sequence directly.  Any other value counts as -1.  NULL: every node follows the one before it.
+ *   lengths (optional): int32 [batch], nodes of each sequence (0 .. nq; outside of that range it counts as the nearer end).
+ *       Rows behind it, and all rows of absent sequences, are not written.
+ *   o must not share memory with q, k, v or the state. */
+#define FASTMAX_TREE_NODES 64
+typedef struct {
+  fastmax_tensor q, k, v;
+  fastmax_tensor o;
+  fastmax_tensor g; /* optional, float32 */
+  fastmax_pages cache;
+  const int32_t* parents;
+  int64_t parents_stride;
+  const int32_t* lengths;
+} fastmax_tree_args;
+int32_t fastmax_tree_attention(const fastmax_problem* pb, const fastmax_tree_args* args, void* cuda_stream);
+
+/* Takes a path of such a tree into the states: S += Phi(k_j)^T [v_j | 1] for j = last, its parent and so on, added from the root down.
+ *   last: int32 [batch], the deepest node of the path; outside 0 .. nk-1: nothing is taken, the state is not touched.
+ *   parents: as above.  pb: nq = nk = nodes per sequence; a0 .. a2, inv_temperature and `causal` are not used.  One launch, no workspace. */
+typedef struct {
+  fastmax_tensor k, v;
+  fastmax_pages cache;
+  const int32_t* parents;
+  int64_t parents_stride;
+  const int32_t* last;
+} fastmax_accept_args;
+int32_t fastmax_tree_accept(const fastmax_problem* pb, const fastmax_accept_args* args, void* cuda_stream);
+
+/* Copies `count` pages of page_floats float32: page dst_index[i] of dst becomes page src_index[i] of src (a NULL index: i itself).  Entries
+ * outside 0 .. pages-1 on either side are left out.  Strides in floats; addresses 16-byte aligned, strides and page_floats multiples of
+ * 4.  No page that is written may be read by the same call or be written twice. */
+typedef struct {
+  const float* src;
+  float* dst;
+  int64_t src_stride, dst_stride, page_floats;
+  int32_t src_pages, dst_pages;
+  const int32_t *src_index, *dst_index;
+  int32_t count;
+  int32_t reserved;
+} fastmax_pages_copy_args;
+int32_t fastmax_pages_copy(const fastmax_pages_copy_args* args, void* cuda_stream);
+
+/* Hands the pages of a cache over between its places: fork, end and begin sequences in one call.
+ *     sources[i] = j, 0 <= j < places : place i goes on from what place j held before the call (nothing, if that was nothing)
+ *     sources[i] = -1                 : place i holds nothing afterwards
+ *     sources[i] = -2                 : place i begins an empty sequence (a page of zeros)
+ * A page from which a place goes on stays with the lowest such place.  Every other place that needs a page takes, in ascending order,
+ * the lowest page that nobody keeps; it is copied there or cleared.  A place that finds none left, or has any other source,
+ * holds nothing (-1) and is counted.
+ *   state: float32 [pages][page_floats]; 16-byte aligned, page_floats a multiple of 4.  table: int32 [places], in and out; entries outside
+ *   0 .. pages-1 mean nothing.  unserved: int32, receives the count.  places, pages: 1 .. FASTMAX_CACHE_PAGES.
+ *   workspace: fastmax_cache_workspace(places) bytes, 16-byte aligned; not to be shared by calls that may overlap.  Two launches. */
+#define FASTMAX_CACHE_PAGES 32768
+size_t fastmax_cache_workspace(int32_t places);
+int32_t fastmax_cache_arrange(float* state, int64_t page_floats, int32_t pages, int32_t* table, int32_t places, const int32_t* sources,
+                              int32_t* unserved, void* workspace, size_t workspace_bytes, void* cuda_stream);
+/* Moves the live pages of a cache to its front: where n pages are live, the m-th live page from position n on (ascending) goes to the m-th
+ * free position before n, and the table follows.  live: int32, receives n.  Everything else as above. */
+int32_t fastmax_cache_compact(float* state, int64_t page_floats, int32_t pages, int32_t* table, int32_t places, int32_t* live,
+                              void* workspace, size_t workspace_bytes, void* cuda_stream);
+
 /* ---- optional key prologue and output epilogue -------------------------------------------------------
  * Two steps the reference's forward_cuda carries but never performs; offered so a caller can switch them on.
  *

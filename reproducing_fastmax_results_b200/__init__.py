@@ -34,7 +34,11 @@ from .attention import (  # noqa: E402
     rpe_matrix_creator,
 )
 
+from .cache import FastmaxCache  # noqa: E402
+from .decoding import FastmaxDecoder  # noqa: E402
+
 __all__ = [
+    "FastmaxCache", "FastmaxDecoder",
     "FastMax", "FASTMultiHeadAttention", "FASTMultiHeadAttention_Function", "fastmax", "fastmax_custom",
     "rpe_matrix_creator", "load_extension",
 ]

@@ -22,7 +22,8 @@ EXPORTED_SYMBOLS = [
     "fastmax_forward_workspace", "fastmax_forward", "fastmax_key_moments_bytes", "fastmax_forward_engine",
     "fastmax_static_scratch_bytes", "fastmax_forward_static_scratch",
     "fastmax_backward_workspace", "fastmax_backward", "fastmax_backward_key_moments_bytes", "fastmax_grad_moments_bytes",
-    "fastmax_decode_step",
+    "fastmax_decode_step", "fastmax_decode_step_paged", "fastmax_tree_attention", "fastmax_tree_accept",
+    "fastmax_pages_copy", "fastmax_cache_workspace", "fastmax_cache_arrange", "fastmax_cache_compact",
     "fastmax_normalize_forward", "fastmax_normalize_backward",
     "fastmax_key_prologue", "fastmax_output_noise",
     "fastmax_status_string", "fastmax_last_cuda_error", "fastmax_last_cuda_error_string",
@@ -73,6 +74,33 @@ class DecodeArgs(C.Structure):
     _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("g", Tensor), ("state", C.c_void_p)]
 
 
+class Pages(C.Structure):
+    _fields_ = [("state", C.c_void_p), ("page_stride", C.c_int64), ("pages", C.c_int32), ("reserved", C.c_int32), ("table", C.c_void_p)]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("g", Tensor), ("cache", Pages)]
+
+
+class TreeArgs(C.Structure):
+    _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("g", Tensor), ("cache", Pages),
+                ("parents", C.c_void_p), ("parents_stride", C.c_int64), ("lengths", C.c_void_p)]
+
+
+class AcceptArgs(C.Structure):
+    _fields_ = [("k", Tensor), ("v", Tensor), ("cache", Pages), ("parents", C.c_void_p), ("parents_stride", C.c_int64), ("last", C.c_void_p)]
+
+
+class PagesCopyArgs(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_stride", C.c_int64), ("dst_stride", C.c_int64), ("page_floats", C.c_int64),
+                ("src_pages", C.c_int32), ("dst_pages", C.c_int32), ("src_index", C.c_void_p), ("dst_index", C.c_void_p),
+                ("count", C.c_int32), ("reserved", C.c_int32)]
+
+
+TREE_NODES = 64   # FASTMAX_TREE_NODES
+CACHE_PAGES = 32768   # FASTMAX_CACHE_PAGES
+
+
 class FastmaxError(RuntimeError):
     def __init__(self, status, what, detail=""):
         self.status = status
@@ -120,6 +148,21 @@ def load():
     lib.fastmax_backward.argtypes = [C.POINTER(Problem), C.POINTER(BackwardArgs), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.fastmax_decode_step.restype = C.c_int32
     lib.fastmax_decode_step.argtypes = [C.POINTER(Problem), C.POINTER(DecodeArgs), C.c_void_p]
+    lib.fastmax_decode_step_paged.restype = C.c_int32
+    lib.fastmax_decode_step_paged.argtypes = [C.POINTER(Problem), C.POINTER(PagedDecodeArgs), C.c_void_p]
+    lib.fastmax_tree_attention.restype = C.c_int32
+    lib.fastmax_tree_attention.argtypes = [C.POINTER(Problem), C.POINTER(TreeArgs), C.c_void_p]
+    lib.fastmax_tree_accept.restype = C.c_int32
+    lib.fastmax_tree_accept.argtypes = [C.POINTER(Problem), C.POINTER(AcceptArgs), C.c_void_p]
+    lib.fastmax_pages_copy.restype = C.c_int32
+    lib.fastmax_pages_copy.argtypes = [C.POINTER(PagesCopyArgs), C.c_void_p]
+    lib.fastmax_cache_workspace.restype = C.c_size_t
+    lib.fastmax_cache_workspace.argtypes = [C.c_int32]
+    lib.fastmax_cache_arrange.restype = C.c_int32
+    lib.fastmax_cache_arrange.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                          C.c_void_p]
+    lib.fastmax_cache_compact.restype = C.c_int32
+    lib.fastmax_cache_compact.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
     lib.fastmax_normalize_forward.restype = C.c_int32
     lib.fastmax_normalize_forward.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float,
                                               C.POINTER(Tensor), C.POINTER(Tensor), C.c_void_p, C.c_void_p]
@@ -342,6 +385,61 @@ def decode_step(q, k, v, state, inv_temp, a0=1.0, a1=1.0, a2=0.5, order=2, out=N
     args.state = state.data_ptr()
     check(lib.fastmax_decode_step(C.byref(pb), C.byref(args), _stream()), "fastmax_decode_step")
     return o, g
+
+
+def _pages(state, table):
+    """(pages, heads, rows, ld) float32 tensor, heads of a page contiguous, and an int32 (batch,) table or None -> fastmax_pages."""
+    assert state.dim() == 4 and state[0].is_contiguous()
+    return Pages(state.data_ptr(), state.stride(0), state.shape[0], 0, None if table is None else table.data_ptr())
+
+
+def decode_step_paged(q, k, v, state, table, inv_temp, a0=1.0, a1=1.0, a2=0.5, order=2, out=None):
+    """Calls fastmax_decode_step_paged: q, k, v are (b, h, d), state a layer of a cache, table int32 (b,).  Returns (o, g), zero where a
+    sequence is absent."""
+    import torch
+
+    lib = load()
+    b, h, d = q.shape
+    o = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    g = torch.zeros((b, h), dtype=torch.float32, device=q.device)
+    pb = Problem(b, h, 1, 1, d, order, 1, dtype_code(q), a0, a1, a2, inv_temp, 0, 0)
+    args = PagedDecodeArgs()
+    args.q, args.k, args.v, args.o = (Tensor(t.data_ptr(), t.stride(0), t.stride(1), 0) for t in (q, k, v, o))
+    args.g = Tensor(g.data_ptr(), g.stride(0), g.stride(1), 0)
+    args.cache = _pages(state, table)
+    check(lib.fastmax_decode_step_paged(C.byref(pb), C.byref(args), _stream()), "fastmax_decode_step_paged")
+    return o, g
+
+
+def tree_attention(q, k, v, state, inv_temp, a0=1.0, a1=1.0, a2=0.5, order=2, table=None, parents=None, lengths=None, out=None):
+    """Calls fastmax_tree_attention on (b, h, n, d) CUDA tensors; table, lengths int32 (b,), parents int32 (b, n).  Returns (o, g), zero in
+    the rows that the call leaves out."""
+    import torch
+
+    lib = load()
+    o = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    g = torch.zeros(q.shape[:3], dtype=torch.float32, device=q.device)
+    pb = problem_for(q, k, True, inv_temp, a0, a1, a2, order)
+    args = TreeArgs()
+    args.q, args.k, args.v, args.o, args.g = view_bhnd(q), view_bhnd(k), view_bhnd(v), view_bhnd(o), view_bhn(g)
+    args.cache = _pages(state, table)
+    if parents is not None:
+        args.parents, args.parents_stride = parents.data_ptr(), parents.stride(0)
+    if lengths is not None:
+        args.lengths = lengths.data_ptr()
+    check(lib.fastmax_tree_attention(C.byref(pb), C.byref(args), _stream()), "fastmax_tree_attention")
+    return o, g
+
+
+def tree_accept(k, v, state, last, order=2, table=None, parents=None):
+    """Calls fastmax_tree_accept on (b, h, n, d) CUDA tensors; last int32 (b,)."""
+    lib = load()
+    pb = problem_for(k, k, True, 1.0, order=order)
+    args = AcceptArgs()
+    args.k, args.v, args.cache, args.last = view_bhnd(k), view_bhnd(v), _pages(state, table), last.data_ptr()
+    if parents is not None:
+        args.parents, args.parents_stride = parents.data_ptr(), parents.stride(0)
+    check(lib.fastmax_tree_accept(C.byref(pb), C.byref(args), _stream()), "fastmax_tree_accept")
 
 
 def normalize_forward(x, lim=1.0):

@@ -20,6 +20,7 @@
 #include "../../include/fastmax_b200.h"
 #include "common.cuh"
 #include "launchers.cuh"
+#include "pages.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -43,6 +44,9 @@ constexpr int UNROLL = 4;   // rows a thread has in flight
 struct DecodeParams {
   View q, k, v, o, g;
   float* state;
+  const int* table;         // page of each sequence, or NULL: heads follow one another without gaps
+  long long page_stride;    // floats
+  int pages;
   int heads, rows;
   float c0, c1, c2;
 };
@@ -89,6 +93,12 @@ decode_step_kernel(const DecodeParams P) {
   }
   grid_wait();   // the step before this one wrote the state
   grid_trigger();
+  long long first = (long long)bi * P.page_stride + (long long)hi * (P.rows * (D + 4));
+  if (P.table != nullptr) {
+    const int page = P.table[bi];
+    if (page < 0 || page >= P.pages) return;   // the whole cluster: an absent sequence
+    first += (long long)(page - bi) * P.page_stride;
+  }
   if (tid < D) {
     const long long off_q = (long long)bi * P.q.sb + (long long)hi * P.q.sh;
     const long long off_k = (long long)bi * P.k.sb + (long long)hi * P.k.sh;
@@ -108,7 +118,7 @@ decode_step_kernel(const DecodeParams P) {
   const int r0 = rank * rows_per;
   const int r1 = min(P.rows, r0 + rows_per);
   const float4 v4 = sv[c4];
-  float4* base = reinterpret_cast<float4*>(P.state) + (long long)head * P.rows * C4 + c4;
+  float4* base = reinterpret_cast<float4*>(P.state + first) + c4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 
   // feature r of k (un-weighted) and of q (weighted)
@@ -261,7 +271,7 @@ static cudaError_t launch_d(int d, int order, const DecodeParams& P, int bh, cud
 }  // namespace dec
 }  // namespace fm
 
-extern "C" int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_decode_args* a, void* cuda_stream) {
+extern "C" int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged_decode_args* a, void* cuda_stream) {
   using namespace fm;
   if (!pb || !a) return FASTMAX_ERR_INVALID_ARGUMENT;
   if (pb->batch <= 0 || pb->heads <= 0) return FASTMAX_ERR_INVALID_ARGUMENT;
@@ -270,15 +280,18 @@ extern "C" int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_
   if (pb->order != 1 && pb->order != 2) return FASTMAX_ERR_UNSUPPORTED;
   if (pb->nq != 1 || pb->nk != 1) return FASTMAX_ERR_UNSUPPORTED;
   if ((long long)pb->batch * pb->heads > 65535) return FASTMAX_ERR_UNSUPPORTED;
-  if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->o.ptr || !a->state) return FASTMAX_ERR_INVALID_ARGUMENT;
-  if (reinterpret_cast<uintptr_t>(a->state) % 16 != 0) return FASTMAX_ERR_MISALIGNED;
+  if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->o.ptr) return FASTMAX_ERR_INVALID_ARGUMENT;
+  if (const int rc = check_pages(pb, a->cache)) return rc;
   dec::DecodeParams P;
   P.q = View{a->q.ptr, a->q.stride_b, a->q.stride_h, a->q.stride_n};
   P.k = View{a->k.ptr, a->k.stride_b, a->k.stride_h, a->k.stride_n};
   P.v = View{a->v.ptr, a->v.stride_b, a->v.stride_h, a->v.stride_n};
   P.o = View{a->o.ptr, a->o.stride_b, a->o.stride_h, a->o.stride_n};
   P.g = View{a->g.ptr, a->g.stride_b, a->g.stride_h, a->g.stride_n};
-  P.state = a->state;
+  P.state = a->cache.state;
+  P.table = a->cache.table;
+  P.page_stride = a->cache.page_stride;
+  P.pages = a->cache.pages;
   P.heads = pb->heads;
   P.rows = state_rows(pb->d, pb->order);
   P.c0 = pb->a0;
@@ -293,4 +306,14 @@ extern "C" int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_
                                   : dec::launch_d<float>(pb->d, pb->order, P, bh, st);
   }
   return e == cudaSuccess ? FASTMAX_OK : report_cuda_error(e);
+}
+
+extern "C" int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_decode_args* a, void* cuda_stream) {
+  if (!pb || !a) return FASTMAX_ERR_INVALID_ARGUMENT;
+  fastmax_paged_decode_args paged{};
+  paged.q = a->q, paged.k = a->k, paged.v = a->v, paged.o = a->o, paged.g = a->g;
+  paged.cache.state = a->state;
+  paged.cache.page_stride = (int64_t)pb->heads * fm::state_rows(pb->d, pb->order) * fm::state_ld(pb->d);
+  paged.cache.pages = pb->batch;
+  return fastmax_decode_step_paged(pb, &paged, cuda_stream);
 }

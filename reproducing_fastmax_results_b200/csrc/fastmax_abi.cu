@@ -55,7 +55,8 @@ static const char* kKindNames[KK_COUNT] = {
     "moments_kv", "moments_qg", "state_scan", "scan_fwd", "scan_bwd_q", "scan_bwd_kv", "finalize_fwd",
     "bwd_prologue", "cast_out", "normalize", "tc_scan_fwd", "tc_scan_bwd_q", "tc_scan_bwd_kv", "tc_moments", "p1_fwd", "tc_intra_fwd", "tc_intra_bwd", "tc_transpose", "tc_scan_bwd_dv", "decode_step", "key_prologue", "output_noise", "tc_pad",
     "pair_fwd", "pair_bwd_q", "pair_bwd_kv", "pair_f32_fwd", "pair_f32_bwd_q", "pair_f32_bwd_kv", "pair_split",
-    "window_pack", "window_fwd", "window_bwd_q", "window_bwd_k", "window_bwd_v"};
+    "window_pack", "window_fwd", "window_bwd_q", "window_bwd_k", "window_bwd_v",
+    "tree_attention", "tree_accept", "cache_plan", "cache_copy"};
 
 int sm_count() {
   static int cached[64] = {0};

@@ -529,6 +529,177 @@ torch::Tensor decode_step(torch::Tensor q, torch::Tensor k, torch::Tensor v, tor
   return o;
 }
 
+// ---- serving: pages of moment states, trees of drafted tokens --------------------------------------------------------
+using maybe = c10::optional<torch::Tensor>;
+bool given(const maybe& t) { return t.has_value() && t->defined(); }
+
+// state: float32 (pages, heads, rows, ld), pages any distance apart (a layer of a cache); table: int32 (batch,) or none
+fastmax_pages pages_of(const torch::Tensor& state, const maybe& table, const fastmax_problem& pb) {
+  CHECK_CUDA(state);
+  const int64_t rows = fastmax_state_rows(pb.d, pb.order), ld = fastmax_state_ld(pb.d);
+  TORCH_CHECK(state.scalar_type() == torch::kFloat32 && state.dim() == 4 && state.size(1) == pb.heads && state.size(2) == rows && state.size(3) == ld &&
+                  state.stride(3) == 1 && state.stride(2) == ld && (pb.heads == 1 || state.stride(1) == rows * ld),
+              "state must be float32 (pages, ", pb.heads, ", ", rows, ", ", ld, ") with the heads of a page contiguous");
+  TORCH_CHECK(state.size(0) <= INT32_MAX, "too many pages");
+  fastmax_pages c{};
+  c.state = (float*)state.data_ptr();
+  c.page_stride = state.size(0) > 1 ? state.stride(0) : pb.heads * rows * ld;
+  c.pages = (int32_t)state.size(0);
+  if (given(table)) {
+    TORCH_CHECK(table->device() == state.device() && table->scalar_type() == torch::kInt32 && table->is_contiguous() && table->dim() == 1 &&
+                    table->size(0) == pb.batch,
+                "table must be a contiguous int32 tensor with one page per sequence, on the state's device");
+    c.table = (const int32_t*)table->data_ptr();
+  } else {
+    TORCH_CHECK(state.size(0) == pb.batch, "without a table the state needs one page per sequence");
+  }
+  return c;
+}
+// int32 (batch,) on the state's device
+const int32_t* per_sequence(const torch::Tensor& t, const fastmax_problem& pb, const torch::Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.dim() == 1 && t.size(0) == pb.batch, name,
+              " must be a contiguous int32 tensor with one entry per sequence, on the state's device");
+  return (const int32_t*)t.data_ptr();
+}
+const int32_t* parents_of(const maybe& parents, const fastmax_problem& pb, const torch::Tensor& like, int64_t& stride) {
+  if (!given(parents)) return nullptr;
+  TORCH_CHECK(parents->device() == like.device() && parents->scalar_type() == torch::kInt32 && parents->dim() == 2 && parents->size(0) == pb.batch &&
+                  parents->size(1) == pb.nq && (pb.nq == 1 || parents->stride(1) == 1),
+              "parents must be an int32 (b, n) tensor with contiguous rows, on the state's device");
+  stride = parents->stride(0);
+  return (const int32_t*)parents->data_ptr();
+}
+// the geometry of (b, h, n, d) tensors of one type on the state's device
+fastmax_problem tree_problem(std::initializer_list<const torch::Tensor*> tensors, const torch::Tensor& state, int64_t p) {
+  const torch::Tensor& first = **tensors.begin();
+  TORCH_CHECK(first.dim() == 4, "q, k, v must be (b, h, n, d)");
+  for (const torch::Tensor* t : tensors) {
+    CHECK_CUDA((*t));
+    TORCH_CHECK(t->device() == state.device(), "the tensors and the state must be on one device");
+    TORCH_CHECK(t->scalar_type() == first.scalar_type(), "dtypes differ");
+    TORCH_CHECK(t->sizes() == first.sizes() && (t->size(3) == 1 || t->stride(3) == 1), "q, k, v and out must be (b, h, n, d) of one size, unit stride on the head dim");
+  }
+  TORCH_CHECK(first.numel() > 0 && first.size(0) <= INT32_MAX && first.size(1) <= INT32_MAX, "q, k, v must not be empty");
+  TORCH_CHECK(first.size(2) <= FASTMAX_TREE_NODES, "at most ", FASTMAX_TREE_NODES, " nodes per sequence");
+  fastmax_problem pb{};
+  pb.batch = first.size(0); pb.heads = first.size(1); pb.nq = pb.nk = first.size(2); pb.d = first.size(3); pb.order = (int)p;
+  pb.causal = 1; pb.dtype = dtype_of(first);
+  TORCH_CHECK((pb.d == 16 || pb.d == 32 || pb.d == 64) && (p == 1 || p == 2), "head dim must be 16, 32 or 64, p 1 or 2");
+  return pb;
+}
+
+torch::Tensor tree_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor state, maybe table, maybe parents, maybe lengths,
+                             double inv_temp, double a0, double a1, double a2, int64_t p, maybe out) {
+  fastmax_problem pb = tree_problem({&q, &k, &v}, state, p);
+  pb.a0 = (float)a0; pb.a1 = (float)a1; pb.a2 = (float)a2; pb.inv_temperature = (float)inv_temp;
+  const c10::cuda::CUDAGuard guard(q.device());
+  fastmax_tree_args a{};
+  a.cache = pages_of(state, table, pb);
+  a.parents = parents_of(parents, pb, state, a.parents_stride);
+  if (given(lengths)) a.lengths = per_sequence(*lengths, pb, state, "lengths");
+  torch::Tensor o;
+  if (given(out)) {
+    o = *out;
+    tree_problem({&q, &o}, state, p);
+  } else {
+    // rows that the call does not write are zero
+    o = a.lengths || a.cache.table ? torch::zeros(q.sizes(), q.options()) : torch::empty(q.sizes(), q.options());
+  }
+  a.q = view_bhnd(q); a.k = view_bhnd(k); a.v = view_bhnd(v); a.o = view_bhnd(o);
+  check_status(fastmax_tree_attention(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax tree_attention");
+  return o;
+}
+
+void tree_accept(torch::Tensor k, torch::Tensor v, torch::Tensor state, torch::Tensor last, maybe table, maybe parents, int64_t p) {
+  fastmax_problem pb = tree_problem({&k, &v}, state, p);
+  const c10::cuda::CUDAGuard guard(k.device());
+  fastmax_accept_args a{};
+  a.cache = pages_of(state, table, pb);
+  a.parents = parents_of(parents, pb, state, a.parents_stride);
+  a.last = per_sequence(last, pb, state, "last");
+  a.k = view_bhnd(k); a.v = view_bhnd(v);
+  check_status(fastmax_tree_accept(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax tree_accept");
+}
+
+torch::Tensor decode_step_paged(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor state, torch::Tensor table, double inv_temp,
+                                double a0, double a1, double a2, int64_t p, maybe out) {
+  CHECK_CUDA(q);
+  TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q, k, v must be (b, h, d) or (b, h, 1, d)");
+  auto rows = [](const torch::Tensor& t) { return t.dim() == 3 ? t.unsqueeze(2) : t; };
+  const torch::Tensor q4 = rows(q), k4 = rows(k), v4 = rows(v);
+  fastmax_problem pb = tree_problem({&q4, &k4, &v4}, state, p);
+  TORCH_CHECK(pb.nq == 1, "one token per (batch, head)");
+  pb.a0 = (float)a0; pb.a1 = (float)a1; pb.a2 = (float)a2; pb.inv_temperature = (float)inv_temp;
+  const c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor o = given(out) ? *out : torch::zeros(q.sizes(), q.options());   // absent sequences' rows are zero
+  const torch::Tensor o4 = rows(o);
+  tree_problem({&q4, &o4}, state, p);
+  fastmax_paged_decode_args a{};
+  a.q = view_bhnd(q4); a.k = view_bhnd(k4); a.v = view_bhnd(v4); a.o = view_bhnd(o4);
+  a.cache = pages_of(state, table, pb);
+  check_status(fastmax_decode_step_paged(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax decode_step");
+  return o;
+}
+
+// state: float32 (pages, ...) contiguous; table, sources: int32 (places,).  Returns int32 (1,): places that could not be served / live pages.
+void check_cache(const torch::Tensor& state, const torch::Tensor& table) {
+  CHECK_INPUT(state);
+  TORCH_CHECK(state.scalar_type() == torch::kFloat32 && state.dim() >= 2 && state.numel() > 0, "state must be float32 (pages, ...)");
+  TORCH_CHECK(table.device() == state.device() && table.scalar_type() == torch::kInt32 && table.dim() == 1 && table.is_contiguous(),
+              "table must be a contiguous int32 (places,) tensor on the state's device");
+  TORCH_CHECK(state.size(0) <= FASTMAX_CACHE_PAGES && table.size(0) >= 1 && table.size(0) <= FASTMAX_CACHE_PAGES, "1 to ", FASTMAX_CACHE_PAGES,
+              " pages and places");
+}
+torch::Tensor cache_arrange(torch::Tensor state, torch::Tensor table, torch::Tensor sources) {
+  check_cache(state, table);
+  TORCH_CHECK(sources.device() == table.device() && sources.scalar_type() == torch::kInt32 && sources.is_contiguous() && sources.sizes() == table.sizes(),
+              "sources must be a contiguous int32 (places,) tensor on the state's device");
+  const c10::cuda::CUDAGuard guard(state.device());
+  const int32_t pages = state.size(0), places = table.size(0);
+  auto unserved = torch::empty({1}, table.options());
+  const size_t need = fastmax_cache_workspace(places);
+  auto ws = workspace(need, state);
+  check_status(fastmax_cache_arrange((float*)state.data_ptr(), state.numel() / pages, pages, (int32_t*)table.data_ptr(), places,
+                                     (const int32_t*)sources.data_ptr(), (int32_t*)unserved.data_ptr(), aligned(ws), need,
+                                     at::cuda::getCurrentCUDAStream().stream()), "fastmax cache_arrange");
+  return unserved;
+}
+torch::Tensor cache_compact(torch::Tensor state, torch::Tensor table) {
+  check_cache(state, table);
+  const c10::cuda::CUDAGuard guard(state.device());
+  const int32_t pages = state.size(0), places = table.size(0);
+  auto live = torch::empty({1}, table.options());
+  const size_t need = fastmax_cache_workspace(places);
+  auto ws = workspace(need, state);
+  check_status(fastmax_cache_compact((float*)state.data_ptr(), state.numel() / pages, pages, (int32_t*)table.data_ptr(), places,
+                                     (int32_t*)live.data_ptr(), aligned(ws), need, at::cuda::getCurrentCUDAStream().stream()), "fastmax cache_compact");
+  return live;
+}
+// page dst_index[i] of dst <- page src_index[i] of src (no index: i itself); float32 (pages, ...), the pages contiguous in themselves
+void pages_copy(torch::Tensor src, torch::Tensor dst, maybe src_index, maybe dst_index, int64_t count) {
+  for (const torch::Tensor* t : {&src, &dst}) {
+    CHECK_CUDA((*t));
+    TORCH_CHECK(t->scalar_type() == torch::kFloat32 && t->dim() >= 2 && t->size(0) > 0 && t->size(0) <= INT32_MAX && t->select(0, 0).is_contiguous(),
+                "pages must be float32 (pages, ...), each of them contiguous");
+  }
+  TORCH_CHECK(src.device() == dst.device() && src.sizes().slice(1) == dst.sizes().slice(1), "source and destination pages must match, on one device");
+  TORCH_CHECK(count >= 0 && count <= INT32_MAX, "count");
+  for (const maybe* t : {&src_index, &dst_index})
+    TORCH_CHECK(!given(*t) || ((*t)->device() == src.device() && (*t)->scalar_type() == torch::kInt32 && (*t)->is_contiguous() && (*t)->numel() == count),
+                "an index must be a contiguous int32 tensor with `count` entries, on the pages' device");
+  const c10::cuda::CUDAGuard guard(src.device());
+  fastmax_pages_copy_args a{};
+  a.src = (const float*)src.data_ptr(); a.dst = (float*)dst.data_ptr();
+  a.page_floats = src.numel() / src.size(0);
+  a.src_stride = src.size(0) > 1 ? src.stride(0) : a.page_floats;
+  a.dst_stride = dst.size(0) > 1 ? dst.stride(0) : a.page_floats;
+  a.src_pages = src.size(0); a.dst_pages = dst.size(0);
+  a.src_index = given(src_index) ? (const int32_t*)src_index->data_ptr() : nullptr;
+  a.dst_index = given(dst_index) ? (const int32_t*)dst_index->data_ptr() : nullptr;
+  a.count = (int32_t)count;
+  check_status(fastmax_pages_copy(&a, at::cuda::getCurrentCUDAStream().stream()), "fastmax pages_copy");
+}
+
 int64_t launch_count() { return (int64_t)fastmax_launch_count(); }
 
 }  // namespace
@@ -554,6 +725,19 @@ PYBIND11_MODULE(fastmax_cuda, m) {
   m.def("decode_step", &decode_step, "one token per (batch, head) against the carried state: returns o", py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("state"), py::arg("inv_temp"), py::arg("a0"), py::arg("a1"), py::arg("a2"), py::arg("p"),
         py::arg("out") = py::none(), release());
+  m.def("decode_step_paged", &decode_step_paged, "decode_step with a page of the state per sequence", py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("state"), py::arg("table"), py::arg("inv_temp"), py::arg("a0"), py::arg("a1"), py::arg("a2"), py::arg("p"),
+        py::arg("out") = py::none(), release());
+  m.def("tree_attention", &tree_attention, "attention of a tree of drafted tokens over the carried state: returns o", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("state"), py::arg("table"), py::arg("parents"), py::arg("lengths"), py::arg("inv_temp"), py::arg("a0"),
+        py::arg("a1"), py::arg("a2"), py::arg("p"), py::arg("out") = py::none(), release());
+  m.def("tree_accept", &tree_accept, "the path to node `last` of a tree is added to the carried state", py::arg("k"), py::arg("v"), py::arg("state"),
+        py::arg("last"), py::arg("table"), py::arg("parents"), py::arg("p"), release());
+  m.def("cache_arrange", &cache_arrange, "pages change hands by `sources`: returns the number of places that found no page", release());
+  m.def("cache_compact", &cache_compact, "live pages move to the front: returns their number", release());
+  m.def("pages_copy", &pages_copy, "pages of src by src_index into pages of dst by dst_index", py::arg("src"), py::arg("dst"), py::arg("src_index"),
+        py::arg("dst_index"), py::arg("count"), release());
+  m.attr("TREE_NODES") = (int)FASTMAX_TREE_NODES;
   m.def("normalize_forward", &normalize_forward, "q/k normalisation: returns [y, stats]", release());
   m.def("normalize_backward", &normalize_backward, "gradient of the q/k normalisation", release());
   m.def("key_prologue", &key_prologue, "k <- k * inv_temp + rpe rows, in place", py::arg("k"), py::arg("inv_temp"),

@@ -23,7 +23,8 @@ enum KernelKind {
   KK_MOMENTS_KV = 0, KK_MOMENTS_QG, KK_STATE_SCAN, KK_SCAN_FWD, KK_SCAN_BWD_Q, KK_SCAN_BWD_KV, KK_FINALIZE,
   KK_PROLOGUE, KK_CAST, KK_NORMALIZE, KK_TC_FWD, KK_TC_BWD_Q, KK_TC_BWD_KV, KK_TC_MOMENTS, KK_P1_FWD, KK_TC_INTRA_FWD, KK_TC_INTRA_BWD, KK_TC_TRANSPOSE, KK_TC_BWD_DV, KK_DECODE, KK_KEY_PROLOGUE, KK_OUTPUT_NOISE, KK_TC_PAD,
   KK_PAIR_FWD, KK_PAIR_BWD_Q, KK_PAIR_BWD_KV, KK_PAIR_F32_FWD, KK_PAIR_F32_BWD_Q, KK_PAIR_F32_BWD_KV, KK_PAIR_SPLIT,   // pairs, whole sequences or windows
-  KK_WINDOW_PACK, KK_WINDOW_FWD, KK_WINDOW_BWD_Q, KK_WINDOW_BWD_K, KK_WINDOW_BWD_V, KK_COUNT                              // states of windows
+  KK_WINDOW_PACK, KK_WINDOW_FWD, KK_WINDOW_BWD_Q, KK_WINDOW_BWD_K, KK_WINDOW_BWD_V,                              // states of windows
+  KK_TREE, KK_TREE_ACCEPT, KK_CACHE_PLAN, KK_CACHE_COPY, KK_COUNT   // serving
 };
 bool profiling_on();   // per-kernel timing is enabled: launch sequences then stay on one stream so the times do not overlap
 void launch_begin(int kind, cudaStream_t st);

@@ -1,0 +1,179 @@
+"""The serving entry points without a GPU: what they refuse before any launch, their Python checks, and the oracle of their tests."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import serving_oracle as so
+from oracle import fastmax_oracle as orc
+from reproducing_fastmax_results_b200 import _lib as L
+from reproducing_fastmax_results_b200.decoding import per_sequence, tree_parents
+
+PTR = 1 << 20   # looks like an aligned address; no refused call reads it
+
+
+def problem(**fields):
+    pb = L.Problem(2, 3, 5, 5, 32, 2, 1, L.FASTMAX_F32, 1.0, 1.0, 0.5, 1.0, 0, 0)
+    for name, value in fields.items():
+        setattr(pb, name, value)
+    return pb
+
+
+def cache(**fields):
+    c = L.Pages(PTR, 3 * 673 * 36, 2, 0, PTR)
+    for name, value in fields.items():
+        setattr(c, name, value)
+    return c
+
+
+def calls(pb, c, missing=None):
+    """The three entry points that read pages, with argument `missing` left out: (name, status)."""
+    lib = L.load()
+    t = L.Tensor(PTR, 3 * 5 * 32, 5 * 32, 32)
+    one = L.PagedDecodeArgs()
+    one.q = one.k = one.v = one.o = t
+    one.cache = c
+    tree = L.TreeArgs()
+    tree.q = tree.k = tree.v = tree.o = t
+    tree.cache = c
+    accept = L.AcceptArgs()
+    accept.k = accept.v = t
+    accept.cache = c
+    accept.last = PTR
+    for args in (one, tree, accept):
+        if missing and hasattr(args, missing):
+            setattr(args, missing, L.Tensor() if isinstance(getattr(args, missing), L.Tensor) else None)
+    single = L.Problem.from_buffer_copy(pb)
+    if pb.nq == pb.nk == 5:
+        single.nq = single.nk = 1
+    yield "step", lib.fastmax_decode_step_paged(C.byref(single), C.byref(one), None)
+    yield "verify", lib.fastmax_tree_attention(C.byref(pb), C.byref(tree), None)
+    yield "accept", lib.fastmax_tree_accept(C.byref(pb), C.byref(accept), None)
+
+
+@pytest.mark.parametrize("fields,status", [
+    ({"batch": 0}, 1), ({"heads": -1}, 1), ({"dtype": 5}, 1), ({"d": 48}, 2), ({"order": 3}, 2), ({"batch": 30000}, 2), ({"nq": 4}, 2), ({"nk": 6}, 2)])
+def test_bad_problems_are_refused(fields, status):
+    for name, got in calls(problem(**fields), cache()):
+        assert got == status, name
+
+
+def test_too_many_nodes_and_none_are_refused():
+    for nodes, status in ((65, 2), (0, 1), (-3, 1)):
+        got = dict(calls(problem(nq=nodes, nk=nodes), cache()))
+        assert got["verify"] == got["accept"] == status and got["step"] == 2
+
+
+@pytest.mark.parametrize("fields,status", [
+    ({"state": None}, 1), ({"pages": 0}, 1), ({"pages": 1, "table": None}, 1), ({"page_stride": 3 * 673 * 36 - 4}, 1), ({"page_stride": 3 * 673 * 36 + 2}, 6),
+    ({"state": PTR + 8}, 6)])
+def test_bad_pages_are_refused(fields, status):
+    for name, got in calls(problem(), cache(**fields)):
+        assert got == status, name
+
+
+@pytest.mark.parametrize("missing,by", [("k", {"step", "verify", "accept"}), ("v", {"step", "verify", "accept"}), ("q", {"step", "verify"}),
+                                        ("o", {"step", "verify"}), ("last", {"accept"})])
+def test_missing_tensors_are_refused(missing, by):
+    # the others would be launched: a misaligned state stops them before that
+    for name, got in calls(problem(), cache(state=PTR + 8), missing):
+        assert got == (1 if name in by else 6), name
+
+
+def test_page_moves_are_refused():
+    lib = L.load()
+    need = lib.fastmax_cache_workspace(7)
+    assert need >= 12 * 7 and lib.fastmax_cache_workspace(0) == 0
+
+    def both(state=PTR, floats=64, pages=9, table=PTR, places=7, sources=PTR, result=PTR, ws=PTR, nbytes=need):
+        return (lib.fastmax_cache_arrange(state, floats, pages, table, places, sources, result, ws, nbytes, None),
+                lib.fastmax_cache_compact(state, floats, pages, table, places, result, ws, nbytes, None) if sources else 1)
+
+    for fields, status in (({"state": None}, 1), ({"table": None}, 1), ({"result": None}, 1), ({"sources": None}, 1), ({"floats": 0}, 1), ({"pages": 0}, 1),
+                           ({"places": 0}, 1), ({"pages": L.CACHE_PAGES + 1}, 2), ({"places": L.CACHE_PAGES + 1}, 2), ({"state": PTR + 4}, 6),
+                           ({"floats": 66}, 6), ({"ws": None}, 3), ({"ws": PTR + 8}, 3), ({"nbytes": need - 1}, 3)):
+        assert both(**fields) == (status, status), fields
+
+    def copy(**fields):
+        a = L.PagesCopyArgs(PTR, 2 * PTR, 64, 64, 64, 4, 4, None, None, 3, 0)
+        for name, value in fields.items():
+            setattr(a, name, value)
+        return lib.fastmax_pages_copy(C.byref(a), None)
+
+    for fields, status in (({"src": None}, 1), ({"dst": None}, 1), ({"page_floats": 0}, 1), ({"src_pages": 0}, 1), ({"dst_pages": -1}, 1), ({"count": -1}, 1),
+                           ({"src_stride": 60}, 1), ({"dst_stride": 0}, 1), ({"src": PTR + 4}, 6), ({"dst": PTR + 8}, 6), ({"src_stride": 66}, 6),
+                           ({"dst_stride": 66}, 6), ({"page_floats": 62}, 6), ({"count": 0}, 0)):
+        assert copy(**fields) == status, fields
+    assert lib.fastmax_pages_copy(None, None) == 1
+
+
+def test_numbers_on_the_host_are_checked():
+    like = torch.zeros(3, 2, 4, 16)
+    assert per_sequence(None, like, "x", 0, 4) is None
+    assert per_sequence([0, 4, 1], like, "x", 0, 4).tolist() == [0, 4, 1]
+    assert per_sequence(torch.tensor([0, 4, 1]), like, "x", 0, 4).dtype == torch.int32
+    for bad, error in (([0, 5, 1], ValueError), ([0, -1, 1], ValueError), ([0, 1], ValueError), (torch.zeros(3), TypeError),
+                       (torch.zeros(3, dtype=torch.bool), TypeError), (torch.zeros(3, 1, dtype=torch.int32), ValueError)):
+        with pytest.raises(error):
+            per_sequence(bad, like, "x", 0, 4)
+    good = torch.tensor([[-1, 0, 0, 2]] * 3)
+    assert tree_parents(None, like) is None and tree_parents(good, like).dtype == torch.int32
+    for bad, error in ((good[:, :3], ValueError), (good[:2], ValueError), (good.float(), TypeError), (torch.tensor([[0, 0, 0, 0]] * 3), ValueError),
+                       (torch.tensor([[-1, 0, 0, 3]] * 3), ValueError), (torch.tensor([[-1, 0, -2, 0]] * 3), ValueError)):
+        with pytest.raises(error):
+            tree_parents(bad, like)
+    with pytest.raises(ValueError):
+        tree_parents(good, like[:, 0])
+
+
+def test_caches_that_cannot_be_are_refused():
+    from reproducing_fastmax_results_b200 import FastmaxCache
+
+    for bad in ({"d": 48}, {"p": 3}, {"places": 0}, {"pages": 0}, {"layers": 0}, {"heads": 0}, {"pages": L.CACHE_PAGES + 1}):
+        with pytest.raises(ValueError):
+            FastmaxCache(**{"places": 2, "heads": 2, "d": 16, "device": "cpu", **bad})
+    cache = FastmaxCache(3, 2, 16, layers=2, pages=5, device="cpu")
+    assert tuple(cache.state.shape) == (5, 2, 2, 209, 20) and cache.table.tolist() == [-1] * 3
+    x = torch.zeros(3, 2, 4, 16)
+    for call in (lambda: cache.begin([0, 0]), lambda: cache.end([3]), lambda: cache.begin([-1]), lambda: cache.arrange([0, 1]), lambda: cache.arrange([0, 3, 1]),
+                 lambda: cache.arrange([0, -3, 1]), lambda: cache.verify(x[:2], x, x), lambda: cache.verify(x, x[:, :1], x), lambda: cache.verify(x, x, x, layer=2),
+                 lambda: cache.verify(x, x, x, lengths=[0, 5, 1]), lambda: cache.accept(x, x, [4, 0, 0]), lambda: cache.accept(x, x, [0, 0, 0], layer=-1),
+                 lambda: cache.step(x[0], x[0], x[0]), lambda: cache.prefill(x, x, x, [0, 1]), lambda: cache.prefill(x, x, x[:, :, :2], [0, 1, 2])):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError):   # there is no CPU path
+        cache.verify(x, x, x)
+
+
+# ---- the oracle ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("order", [1, 2])
+@pytest.mark.parametrize("d", [16, 32])
+def test_tree_oracle_is_the_operator_on_every_path(d, order):
+    """What a node gets is the last row of the causal operator over the sequence and the node's path."""
+    rng = np.random.default_rng(d + order)
+    n, before = 9, 20
+    a, inv_t = (1.1, 0.9, 0.4), 0.2
+    k0, v0 = rng.standard_normal((2, before, d))
+    q, k, v = rng.standard_normal((3, n, d))
+    parents = [-1, 0, 0, 1, -1, 4, 2, 2, 5]
+    state, _ = so.grown(np.zeros((so.features(k0[:1], order).shape[1], d + 4)), k0, v0, order)
+    state = np.concatenate([state, np.zeros((len(state), 3))], 1)
+    o, g, _, _ = so.tree(q, k, v, state, parents, order, a, inv_t)
+    poly = orc.Poly(*a, inv_t, order)
+    for i in range(n):
+        nodes = so.path(parents, i)
+        keys, values = np.concatenate([k0, k[nodes]]), np.concatenate([v0, v[nodes]])
+        o_ref, g_ref = orc.fastmax_naive(q[i][None, None, None], keys[None, None], values[None, None], False, poly)
+        assert np.allclose(o[i], o_ref[0, 0, 0], rtol=1e-11, atol=1e-11) and np.isclose(g[i], g_ref[0, 0, 0], rtol=1e-11)
+
+
+def test_page_oracle():
+    table = [3, -1, 0, 2]
+    assert so.arranged(table, [0, 1, 2, 3], 4) == ([3, -1, 0, 2], [], 0)
+    assert so.arranged(table, [2, 0, 2, -1], 4) == ([0, 3, 1, -1], [(0, 1)], 0)
+    assert so.arranged(table, [-2, 2, 2, 2], 4) == ([1, 0, 2, 3], [(-1, 1), (0, 2), (0, 3)], 0)
+    assert so.arranged(table, [-2, 9, -3, 3], 2) == ([0, -1, -1, -1], [(-1, 0)], 2)
+    assert so.arranged([0, 1], [0, -2], 1) == ([0, -1], [], 1)
+    assert so.compacted([3, -1, 5, 0], 6) == ([1, -1, 2, 0], [(3, 1), (5, 2)], 3)
+    assert so.compacted([-1, -1], 3) == ([-1, -1], [], 0)
