@@ -1422,7 +1422,8 @@ int tc_wait_histogram(int* out, int n) {
   for (int i = 0; i < n; ++i) out[i] = i < 256 ? h[i] : 0;
   static const int zeros[256] = {0};
   cudaMemcpyToSymbol(g_tc_wait_hist, zeros, sizeof(zeros), 0, cudaMemcpyHostToDevice);
-  return pair_wait_histogram(out, n);
+  const int rc = pair_wait_histogram(out, n);
+  return rc != FASTMAX_OK ? rc : tree_wait_histogram(out, n);
 }
 
 int tc_device_status(int* out) {
@@ -1438,6 +1439,10 @@ int tc_device_status(int* out) {
   const int rc = pair_status(&p);
   if (rc != FASTMAX_OK) return rc;
   if (v == 0) *out = p;
+  int t = 0;
+  const int rt = tree_status(&t);
+  if (rt != FASTMAX_OK) return rt;
+  if (*out == 0) *out = t;
   return FASTMAX_OK;
 }
 

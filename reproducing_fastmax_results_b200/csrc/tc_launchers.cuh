@@ -24,6 +24,8 @@ int tc_forward(const fastmax_problem* pb, const fastmax_forward_args* a, void* w
 int tc_backward(const fastmax_problem* pb, const fastmax_backward_args* a, void* ws, size_t ws_bytes, cudaStream_t st);
 // Reads (and clears) the device-side error word the bounded waits of the tensor-core kernels set.
 int tc_device_status(int* out);
+int tree_status(int* out);                  // tree.cu: included in the two of this file
+int tree_wait_histogram(int* out, int n);
 // Copies (and clears) the per-wait-site give-up counters (index = error code & 255).
 int tc_wait_histogram(int* out, int n);
 // Launches the test-only kernel that lets a bounded wait of `cycles` SM clocks run out and records wait site `code`.

@@ -4,11 +4,14 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/fastmax_b200.h"
 #include "common.cuh"
 #include "launchers.cuh"
 #include "pages.cuh"
+#include "tc_launchers.cuh"
+#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -18,6 +21,29 @@ int report_cuda_error(cudaError_t e);
 int sm_count();
 
 namespace tree {
+
+using namespace tc;
+
+__device__ int g_status = 0;       // see tc_device_status
+__device__ int g_wait_hist[256];
+
+constexpr long long WAIT_CYCLES = 4000000000ll;   // ~2 s at 2 GHz
+
+// Waits for the phase of parity `parity`.  Returns in any case: when the wait runs out (code `code`), the flag is up, no further copy is
+// asked for and every later wait of the block falls through at once.
+__device__ __noinline__ void wait_slow(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
+  if (*abort_flag == 0 && !mbar_wait_abortable(bar, parity, WAIT_CYCLES, abort_flag)) {
+    if (*abort_flag == 0) atomicAdd(&g_wait_hist[code & 255], 1);
+    *abort_flag = 1;
+    atomicExch(&g_status, code);
+  }
+}
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
+  // (a test that does not suspend the thread: waking it costs some 250 clocks, and the copy has mostly arrived)
+  for (int i = 0; i < 64; ++i)
+    if (mbar_test_wait(bar, parity)) return;
+  wait_slow(bar, parity, code, abort_flag);
+}
 
 struct TreeParams {
   View q, k, v, o, g;
@@ -46,16 +72,38 @@ __device__ __forceinline__ void load4v(const float* p, bool aligned, float (&x)[
     for (int i = 0; i < 4; ++i) x[i] = p[i];
   }
 }
-__device__ __forceinline__ void load4v(const __nv_bfloat16* p, bool aligned, float (&x)[4]) {
-  if (aligned) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+// the same in two steps: what is in flight, and its floats
+template <typename T>
+struct Raw4;
+template <>
+struct Raw4<float> {
+  float4 v;
+  __device__ __forceinline__ void load(const float* p, bool aligned) {
+    float x[4];
+    load4v(p, aligned, x);
+    v = make_float4(x[0], x[1], x[2], x[3]);
   }
-}
+  __device__ __forceinline__ void get(bool there, float (&x)[4]) const {
+    x[0] = there ? v.x : 0.f, x[1] = there ? v.y : 0.f, x[2] = there ? v.z : 0.f, x[3] = there ? v.w : 0.f;
+  }
+};
+template <>
+struct Raw4<__nv_bfloat16> {
+  uint2 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, bool aligned) {
+    if (aligned) {
+      v = *reinterpret_cast<const uint2*>(p);
+    } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+      v = make_uint2(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16);
+    }
+  }
+  __device__ __forceinline__ void get(bool there, float (&x)[4]) const {
+    const uint32_t a = there ? v.x : 0u, b = there ? v.y : 0u;
+    x[0] = __uint_as_float(a << 16), x[1] = __uint_as_float(a & 0xffff0000u);
+    x[2] = __uint_as_float(b << 16), x[3] = __uint_as_float(b & 0xffff0000u);
+  }
+};
 __device__ __forceinline__ void store4v(float* p, bool aligned, float a, float b, float c, float d) {
   if (aligned) {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
@@ -124,111 +172,161 @@ __device__ __forceinline__ uint32_t twice(uint32_t x) {   // of two bfloat16, ex
   const __nv_bfloat162 r = __hadd2(v, v);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ int count_up(int* counter) {   // in shared memory; orders what the warps did before
+  int old;
+  asm volatile("atom.add.acq_rel.cta.shared::cta.s32 %0, [%1], 1;" : "=r"(old) : "r"(smem_u32(counter)) : "memory");
+  return old;
+}
+// c += s * p, the two halves of 64 bits each
+__device__ __forceinline__ void fma2(float& c0, float& c1, float2 s, float p0, float p1) {
+  asm("{\n\t.reg .b64 c, s, p;\n\t"
+      "mov.b64 c, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tmov.b64 p, {%4, %5};\n\t"
+      "fma.rn.f32x2 c, s, p, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(c0), "+f"(c1) : "f"(s.x), "f"(s.y), "f"(p0), "f"(p1));
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
+__device__ __forceinline__ void mma16816_from_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// a product of 16 terms from the pieces of the state and of x, the smallest first
+template <int SP, int QP>
+__device__ __forceinline__ void products(float (&c)[4], const uint32_t (&a)[SP][4], const uint32_t (&x)[2][QP]) {
+#pragma unroll
+  for (int p = SP - 1; p >= 0; --p)
+#pragma unroll
+    for (int i = 0; i <= p; ++i)
+      if (p - i < QP) {
+        if (p == SP - 1 && i == (p < QP ? 0 : p - QP + 1)) mma16816_from_zero(c, a[i], x[0][p - i], x[1][p - i]);
+        else mma16816(c, a[i], x[0][p - i], x[1][p - i]);
+      }
+}
 
 template <typename T, int D, int NT>
 struct TreeGeo {
-  static constexpr int WARPS = NT == 8 && D > 16 ? 16 : 8;
-  static constexpr int THREADS = 32 * WARPS;
-  static constexpr int BLOCKS = NT == 8 ? 1 : 2;       // to an SM
   static constexpr int N = 8 * NT;                     // nodes, filled up
   static constexpr int NB = D / 8;
-  static constexpr int MT = D / 16;                    // tiles of 16 state columns
-  static constexpr int KG = WARPS / MT;                // groups of warps that share a tile and take turns with the rows m
+  static constexpr int CG = D / 16;                    // groups of 16 columns of the state: one to a warp
+  static constexpr int KG = NT == 8 || D < 64 ? (D == 16 ? 8 : 4) : 2;   // warps that share a group and divide the rows m of a block among them
   static constexpr int RI = 8 / KG;
+  static constexpr int WARPS = CG * KG;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int BLOCKS = NT == 8 ? 1 : 2;       // to an SM
   static constexpr int LDS = D + 4, C4 = LDS / 4;
-  static constexpr int LQ = D + 8;                     // rows of x pieces: fragments without bank conflicts
+  static constexpr int LQ = D + 8;                     // rows of pieces: fragments without bank conflicts
   static constexpr int UNIT = 64 * LDS;                // floats
   static constexpr int QP = Pieces<T>::Q, SP = Pieces<T>::S;
-  // shared memory in bytes; the slots also hold the partial sums at the end
+  static constexpr bool HOLD = 2 * NT * QP <= 16;      // a step's fragments of x stay in registers
+  // shared memory in bytes; the place of keys, values and their weights also takes the warps' sums at the end
   static constexpr int PIECES = QP * N * LQ * 2;
   static constexpr int SCALES = D * N * 4;
   static constexpr int ROWS = N * LDS * 4;
-  static constexpr int WEIGHTS = N * N * 4;
-  static constexpr int FIXED = PIECES + SCALES + 3 * ROWS + WEIGHTS + N * 16;
-  static constexpr int SLOT = 2 * UNIT * 4;
-  static constexpr int RED = KG * ROWS + WARPS * N * 4;
+  static constexpr int TREE = PIECES + ROWS + N * N * 4;
+  static constexpr int SUMS = KG * ROWS;
+  static constexpr int SHARED = TREE > SUMS ? TREE : SUMS;
+  static constexpr int FIXED = PIECES + SCALES + ROWS + SHARED + N * 8 + 256;
+  static constexpr int SLOT = (D == 16 ? 64 : D + 1 > 64 ? D + 1 : 64) * LDS * 4;   // a unit, or the linear rows
   static constexpr int ROOM = (BLOCKS == 2 ? 113 : 227) * 1024 - FIXED;
-  static constexpr int SLOTS = ROOM / SLOT < 2 ? 2 : ROOM / SLOT > 5 ? 5 : ROOM / SLOT;
-  static constexpr int BYTES = FIXED + (SLOTS * SLOT > RED ? SLOTS * SLOT : RED);
-  static_assert(KG * MT == WARPS && RI * KG == 8);
+  static constexpr int SLOTS = ROOM / SLOT > 8 ? 8 : ROOM / SLOT;
+  static constexpr int BYTES = FIXED + SLOTS * SLOT;
+  static_assert(SLOTS >= 3);
 };
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(TreeGeo<T, D, NT>::THREADS, TreeGeo<T, D, NT>::BLOCKS)
 attention_kernel(const TreeParams P) {
   using G = TreeGeo<T, D, NT>;
-  constexpr int N = G::N, LDS = G::LDS, C4 = G::C4, QP = G::QP, SP = G::SP, THREADS = G::THREADS, NB = G::NB;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem);                       // [QP][N][LQ]
-  float* sX = reinterpret_cast<float*>(smem + G::PIECES);                           // [D][N]: x, transposed
-  float* sK = sX + D * N;                                                           // [N][LDS]
-  float* sV = sK + N * LDS;                                                         // [N][LDS]: [v | 1 0 0 0]
-  float* sT = sV + N * LDS;                                                         // [N][LDS]: the tree's own sums, then the results
-  float* sW = sT + N * LDS;                                                         // [N][N]: f of the nodes' pairs
-  unsigned long long* sA = reinterpret_cast<unsigned long long*>(sW + N * N);       // [N]: ancestors
-  int* sP = reinterpret_cast<int*>(sA + N);                                         // [N]
-  float* slots = reinterpret_cast<float*>(smem + G::FIXED);                         // [SLOTS][2 UNIT]
+  constexpr int N = G::N, LDS = G::LDS, C4 = G::C4, LQ = G::LQ, QP = G::QP, SP = G::SP, NB = G::NB, KG = G::KG, RI = G::RI, SLOTS = G::SLOTS, THREADS = G::THREADS;
+  extern __shared__ __align__(128) unsigned char smem[];
+  // [SLOTS][SLOT] units of the state, then
+  __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem + SLOTS * G::SLOT);     // [QP][N][LQ]: pieces of x
+  float* sX = reinterpret_cast<float*>(smem + SLOTS * G::SLOT + G::PIECES);         // [D][N]: x, transposed
+  float* sT = sX + D * N;                                                           // [N][LDS]: the tree's own sums, then the results
+  float* sV = sT + N * LDS;                                                         // [N][LDS]
+  float* sW = sV + N * LDS;                                                         // [N][N]: f of the nodes' pairs
+  __nv_bfloat16* sK = reinterpret_cast<__nv_bfloat16*>(sW + N * N);                 // [QP][N][LQ]: pieces of the keys
+  float* part = sV;                                                                 // [KG][N][LDS], in the place of these three
+  unsigned long long* sA = reinterpret_cast<unsigned long long*>(sV + G::SHARED / 4);   // [N]: ancestors
+  uint64_t* full = reinterpret_cast<uint64_t*>(sA + N);                                                          // [SLOTS]: a slot's copy has arrived
+  int* through = reinterpret_cast<int*>(full + 8);                                  // [SLOTS]: warps that are done with it
+  volatile int* issued = reinterpret_cast<volatile int*>(through + 8);              // [SLOTS]: copies that were asked for
+  volatile int* abort_flag = issued + 8;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster.block_rank(), CL = (int)gridDim.x;
-  const int head = blockIdx.y, b = head / P.heads, h = head - b * P.heads;
+  const int head = blockIdx.y, b = head / P.heads;
+  const int npairs = P.order == 2 ? Geo<D>::NPAIRS : 0;
+  if (tid == 0) {
+    for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1), through[i] = 0, issued[i] = 0;
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  auto meet = [&]() {
+    if (CL > 1) cluster.sync();
+    else __syncthreads();
+  };
   grid_wait();
   grid_trigger();
-  const float* S = head_state(P, b, h, D);
-  const int n = P.ends == nullptr ? P.nodes : min(max(P.ends[b], 0), P.nodes);
-  if (S == nullptr || n == 0) return;   // the whole cluster
-
-  // ---- this block's steps: one or two units (a, b), (a, b + 1), then the linear rows -------------------------------------------
-  const int npairs = P.order == 2 ? Geo<D>::NPAIRS : 0;
-  const int u_first = rank * (npairs + 1) / CL, u_end = (rank + 1) * (npairs + 1) / CL;   // the linear rows are the last unit
-  auto row_of = [&](int u, int& a, int& bb) {
-    if (u < npairs) pair_decode(u, NB, a, bb);
-    else a = bb = NB;
-  };
-  auto units_of = [&](int u, int bb) { return u < npairs ? min(min(2, NB - bb), min(u_end, npairs) - u) : 1; };
-  int lu = u_first, la, lb;   // next step to load
-  row_of(lu, la, lb);
-  auto load_step = [&](int slot) {
-    if (lu < u_end) {
-      const int count = units_of(lu, lb);
-      const int quads = (lu < npairs ? count * 64 : D + 1) * C4;
-      const float4* src = reinterpret_cast<const float4*>(S) + (long long)lu * 64 * C4;
-      float4* dst = reinterpret_cast<float4*>(slots + slot * 2 * G::UNIT);
-      for (int i = tid; i < quads; i += THREADS) copy16_async(dst + i, src + i);
-      lu += count, lb += count;
-      if (lb >= NB) ++la, lb = la;
-    }
-    copies_commit();
-  };
-#pragma unroll
-  for (int i = 0; i + 1 < G::SLOTS; ++i) load_step(i);
-
-  // ---- x, keys, values --------------------------------------------------------------------------------------------------------
+  // Queries, keys and values of all rows that the tensors have are asked for at once, before it is known which of them count: what comes
+  // behind the copies of the state waits for those.
+  constexpr int ITEMS = (N * (D / 4) + THREADS - 1) / THREADS;
+  Raw4<T> rq[ITEMS], rk[ITEMS], rv[ITEMS];
   {
     const T* q = head_base<T>(P.q, head, P.heads);
     const T* k = head_base<T>(P.k, head, P.heads);
     const T* v = head_base<T>(P.v, head, P.heads);
-    for (int idx = tid; idx < N * (D / 4); idx += THREADS) {
-      const int i = idx / (D / 4), c = 4 * (idx - i * (D / 4));
-      float x[4] = {}, y[4] = {}, z[4] = {};
-      if (i < n) {
-        load4v(q + i * P.q.sn + c, P.aligned, x);
-        load4v(k + i * P.k.sn + c, P.aligned, y);
-        load4v(v + i * P.v.sn + c, P.aligned, z);
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) {
+      const int idx = tid + t * THREADS, i = idx / (D / 4), c = 4 * (idx - i * (D / 4));
+      if (i < P.nodes) {
+        rq[t].load(q + i * P.q.sn + c, P.aligned);
+        rk[t].load(k + i * P.k.sn + c, P.aligned);
+        rv[t].load(v + i * P.v.sn + c, P.aligned);
       }
-      *reinterpret_cast<float4*>(sK + i * LDS + c) = make_float4(y[0], y[1], y[2], y[3]);
+    }
+  }
+  const float* S = head_state(P, b, head - b * P.heads, D);
+  const int n = P.ends == nullptr ? P.nodes : min(max(P.ends[b], 0), P.nodes);
+  if (S == nullptr || n == 0) return;   // the whole cluster
+
+  // This block's units of the state: pairs of blocks (a, b), at the end the linear rows as one.
+  const int u_first = rank * (npairs + 1) / CL, u_end = (rank + 1) * (npairs + 1) / CL;
+  auto load = [&](int i) {
+    const int slot = i % SLOTS, u = u_first + i;
+    const uint32_t bytes = (u < npairs ? 64 : D + 1) * LDS * 4;
+    issued[slot] = i / SLOTS + 1;
+    mbar_arrive_expect_tx(&full[slot], bytes);
+    bulk_load(smem + slot * G::SLOT, S + (long long)u * G::UNIT, bytes, &full[slot]);
+  };
+  if (tid == 0)
+    for (int i = 0; i < SLOTS && u_first + i < u_end; ++i) load(i);
+  unsigned long long seen[2];   // of nodes lane and lane + 32: warp 0 finds out who sees whom
+  int up[2];
+  if (warp == 0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = lane + 32 * k;
+      seen[k] = P.parents == nullptr ? (2ull << i) - 1ull : 1ull << i;
+      up[k] = P.parents == nullptr || i >= n ? -1 : parent_of(P, b, i);
+    }
+  }
+
+  // ---- x, keys, values ----------------------------------------------------------------------------------------------------------
+  {
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) {
+      const int idx = tid + t * THREADS, i = idx / (D / 4), c = 4 * (idx - i * (D / 4));
+      if (i >= N) continue;
+      float x[4], y[4], z[4];
+      rq[t].get(i < n, x);
+      rk[t].get(i < n, y);
+      rv[t].get(i < n, z);
       *reinterpret_cast<float4*>(sV + i * LDS + c) = make_float4(z[0], z[1], z[2], z[3]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sX[(c + j) * N + i] = x[j];
@@ -236,281 +334,293 @@ attention_kernel(const TreeParams P) {
       split2(x[0], x[1], p0);
       split2(x[2], x[3], p1);
 #pragma unroll
-      for (int p = 0; p < QP; ++p) *reinterpret_cast<uint2*>(sQ + (p * N + i) * G::LQ + c) = make_uint2(p0[p], p1[p]);
-    }
-    for (int i = tid; i < N; i += THREADS) {
-      *reinterpret_cast<float4*>(sV + i * LDS + D) = make_float4(1.f, 0.f, 0.f, 0.f);
-      sA[i] = P.parents == nullptr ? (2ull << i) - 1ull : 1ull << i;
-      sP[i] = P.parents == nullptr || i >= n ? -1 : parent_of(P, b, i);
+      for (int p = 0; p < QP; ++p) *reinterpret_cast<uint2*>(sQ + (p * N + i) * LQ + c) = make_uint2(p0[p], p1[p]);
+      split2(y[0], y[1], p0);
+      split2(y[2], y[3], p1);
+#pragma unroll
+      for (int p = 0; p < QP; ++p) *reinterpret_cast<uint2*>(sK + (p * N + i) * LQ + c) = make_uint2(p0[p], p1[p]);
     }
   }
-  __syncthreads();
-  if (P.parents != nullptr) {   // pointers twice as far up in every round
-    for (int far = 1; far < n; far *= 2) {
-      unsigned long long seen = 0;
-      int up = -1;
-      if (tid < N && sP[tid] >= 0) seen = sA[sP[tid]], up = sP[sP[tid]];
-      __syncthreads();
-      if (tid < N) sA[tid] |= seen, sP[tid] = up;
-      __syncthreads();
-    }
-  }
-  // ---- the tree: this block's share of the nodes, by CUDA cores: only what a node sees is touched -----------------------------
-  const int per = (n + CL - 1) / CL, i0 = min(n, rank * per), mine = min(n, i0 + per) - i0;
-  const int jgroups = (n + 3) / 4;
-  for (int idx = tid; idx < mine * jgroups; idx += THREADS) {
-    const int j = 4 * (idx / mine), i = i0 + idx % mine;
-    if (((sA[i] >> j) & 15ull) == 0) continue;
-    float dot[4] = {};
-#pragma unroll 4
-    for (int m = 0; m < D; m += 4) {
-      float x[4];
+  if (warp == 0) {
+    if (P.parents != nullptr) {
+      for (int far = 1; far < n; far *= 2) {   // pointers twice as far up in every round
+        unsigned long long more[2];
+        int next[2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) x[t] = sX[(m + t) * N + i];
+        for (int k = 0; k < 2; ++k) {
+          const unsigned long long m0 = __shfl_sync(0xffffffffu, seen[0], up[k] & 31), m1 = __shfl_sync(0xffffffffu, seen[1], up[k] & 31);
+          const int n0 = __shfl_sync(0xffffffffu, up[0], up[k] & 31), n1 = __shfl_sync(0xffffffffu, up[1], up[k] & 31);
+          more[k] = up[k] < 0 ? 0ull : up[k] < 32 ? m0 : m1;
+          next[k] = up[k] < 0 ? -1 : up[k] < 32 ? n0 : n1;
+        }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float4 y = *reinterpret_cast<const float4*>(sK + (j + t) * LDS + m);
-        dot[t] = fmaf(x[0], y.x, fmaf(x[1], y.y, fmaf(x[2], y.z, fmaf(x[3], y.w, dot[t]))));
+        for (int k = 0; k < 2; ++k) seen[k] |= more[k], up[k] = next[k];
       }
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const float s = dot[t] * P.inv_t;
-      sW[(i - i0) * N + j + t] = P.a0 + s * (P.a1 + (P.order == 2 ? P.a2 * s : 0.f));
+    for (int k = 0; k < 2; ++k)
+      if (lane + 32 * k < N) sA[lane + 32 * k] = seen[k];
+  }
+  const int g = lane >> 2, t2 = 2 * (lane & 3);
+  auto x_pieces = [&](uint32_t (&out)[QP], int nt, int m, bool doubled) {
+#pragma unroll
+    for (int p = 0; p < QP; ++p) {
+      out[p] = *reinterpret_cast<const uint32_t*>(sQ + (p * N + 8 * nt + g) * LQ + m + t2);
+      if (doubled) out[p] = twice(out[p]);   // a block off the diagonal stands for two
+    }
+  };
+  __syncthreads();
+  // ---- the tree: this block's share of the nodes ----------------------------------------------------------------------------------
+  // Scores are products of keys (rows) and x (columns); each depends on its own pair alone.  The sums over the ancestors touch only what a
+  // node sees, by CUDA cores: an infinity or NaN in another branch stays there.
+  const int per = (n + CL - 1) / CL, i0 = min(n, rank * per), mine = min(n, i0 + per) - i0;
+  {
+    const int nt0 = i0 / 8, nt1 = (i0 + mine + 7) / 8, jts = (n + 15) / 16;
+    for (int w = warp; w < (nt1 - nt0) * jts; w += G::WARPS) {
+      const int jt = w % jts, nt = nt0 + w / jts;
+      if (16 * jt > 8 * nt + 7) continue;   // nobody of them is an ancestor
+      float c[4] = {};
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t a[QP][4], x[2][QP];
+#pragma unroll
+        for (int p = 0; p < QP; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * jt + g + 8 * (r & 1);   // (with one tile of eight nodes the lower rows do not exist)
+            a[p][r] = j < N ? *reinterpret_cast<const uint32_t*>(sK + (p * N + j) * LQ + 16 * ks + 8 * (r >> 1) + t2) : 0u;
+          }
+        x_pieces(x[0], nt, 16 * ks, false);
+        x_pieces(x[1], nt, 16 * ks + 8, false);
+        float d[4];
+        products(d, a, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] += d[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + g + 8 * (r >> 1), i = 8 * nt + t2 + (r & 1);
+        const float s = c[r] * P.inv_t;
+        if (j < N) sW[i * N + j] = P.a0 + s * (P.a1 + (P.order == 2 ? P.a2 * s : 0.f));
+      }
     }
   }
   __syncthreads();
-  for (int idx = tid; idx < mine * C4; idx += THREADS) {
-    const int i = idx / C4, c = 4 * (idx - i * C4);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (unsigned long long left = sA[i0 + i]; left != 0; left &= left - 1) {
-      const int j = __ffsll((long long)left) - 1;
-      const float w = sW[i * N + j];
-      const float4 y = *reinterpret_cast<const float4*>(sV + j * LDS + c);
-      acc.x = fmaf(w, y.x, acc.x), acc.y = fmaf(w, y.y, acc.y), acc.z = fmaf(w, y.z, acc.z), acc.w = fmaf(w, y.w, acc.w);
+  for (int idx = tid; idx < mine * (D / 4); idx += THREADS) {
+    const int i = idx / (D / 4), c = 4 * (idx - i * (D / 4));
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.f;
+    for (unsigned long long left = sA[i0 + i]; left != 0;) {
+      float w[4];
+      float4 y[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {   // four nodes' loads at a time
+        w[t] = 0.f, y[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (left != 0) {
+          const int j = __ffsll((long long)left) - 1;
+          left &= left - 1;
+          w[t] = sW[(i0 + i) * N + j];
+          y[t] = *reinterpret_cast<const float4*>(sV + j * LDS + c);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        sum.x = fmaf(w[t], y[t].x, sum.x), sum.y = fmaf(w[t], y[t].y, sum.y), sum.z = fmaf(w[t], y[t].z, sum.z), sum.w = fmaf(w[t], y[t].w, sum.w);
+        total += w[t];
+      }
     }
-    *reinterpret_cast<float4*>(sT + i * LDS + c) = acc;   // read by this thread alone
+    *reinterpret_cast<float4*>(sT + i * LDS + c) = sum;
+    if (c == 0) *reinterpret_cast<float4*>(sT + i * LDS + D) = make_float4(total, 0.f, 0.f, 0.f);
   }
 
   // ---- the state --------------------------------------------------------------------------------------------------------------
-  const int mt = warp % G::MT, kg = warp / G::MT;
-  const int g = lane >> 2, t2 = 2 * (lane & 3);
+  const int kg = warp / G::CG, column = 16 * (warp % G::CG) + 2 * g;   // this warp's rows m, this thread's two columns
+  const float c1 = P.a1 * P.inv_t, c2 = P.a2 * P.inv_t * P.inv_t;
   float acc[NT][4] = {}, den[NT][2] = {};
-  // products of 16 terms: `a` the pieces of the state, b0 / b1 those of x
-  auto products = [&](float (&c)[4], const uint32_t (&a)[SP][4], const uint32_t (&b0)[QP], const uint32_t (&b1)[QP]) {
-#pragma unroll
-    for (int p = QP + SP - 2; p >= 0; --p)   // the smallest first
-#pragma unroll
-      for (int i = 0; i < SP; ++i)
-        if (p - i >= 0 && p - i < QP && p < SP) mma16816(c, a[i], b0[p - i], b1[p - i]);
-  };
-  auto x_pieces = [&](uint32_t (&out)[QP], int node, int m) {
-#pragma unroll
-    for (int p = 0; p < QP; ++p) out[p] = *reinterpret_cast<const uint32_t*>(sQ + (p * N + node) * G::LQ + m);
-  };
-  // pieces of rows r, r + 1 (terms 0..7 of two threads' rows) of one column
-  auto s_pieces = [&](uint32_t (&a)[SP][4], int reg, const float* at, int ld) {
+  // pieces of two rows of two columns (of the product: rows g and g + 8)
+  auto s_pieces = [&](uint32_t (&a)[SP][4], int half, const float* at) {
+    const float2 x = *reinterpret_cast<const float2*>(at), y = *reinterpret_cast<const float2*>(at + LDS);
     uint32_t p[SP];
-    split2(at[0], at[ld], p);
+    split2(x.x, y.x, p);
 #pragma unroll
-    for (int i = 0; i < SP; ++i) a[i][reg] = p[i];
+    for (int k = 0; k < SP; ++k) a[k][2 * half] = p[k];
+    split2(x.y, y.y, p);
+#pragma unroll
+    for (int k = 0; k < SP; ++k) a[k][2 * half + 1] = p[k];
   };
-
-  int u = u_first, ua, ub, slot = 0, step = 0;
-  row_of(u, ua, ub);
-  while (u < u_end) {
-    copies_wait<G::SLOTS - 2>();
-    __syncthreads();   // the step has arrived; everybody is done with the slot before it
-    load_step(slot == 0 ? G::SLOTS - 1 : slot - 1);
-    const float* U = slots + slot * 2 * G::UNIT;
-    if (u < npairs) {
-      const int count = units_of(u, ub);
-      // (the second unit of a step without one: zeros)
+  auto last_pieces = [&](uint32_t (&a)[SP][4], int half, const float* at) {
+    uint32_t p[SP];
+    split2(at[0], at[LDS], p);
 #pragma unroll
-      for (int r = 0; r < G::RI; ++r) {
-        const int mi = kg * G::RI + r;
-        const float* row = U + (8 * mi + t2) * LDS + 16 * mt + g;
-        uint32_t a[SP][4];
-        s_pieces(a, 0, row, LDS);
-        s_pieces(a, 1, row + 8, LDS);
-        if (count == 2) {
-          s_pieces(a, 2, row + G::UNIT, LDS);
-          s_pieces(a, 3, row + G::UNIT + 8, LDS);
-        } else {
+    for (int k = 0; k < SP; ++k) a[k][2 * half] = p[k];
+  };
+  int ua = NB, ub = NB, step = 0;
+  if (u_first < npairs) pair_decode(u_first, NB, ua, ub);
+  // one or two units of a block row for the tiles of eight nodes that there are: straight code for each number of them
+  auto pair_step = [&](auto tiles, const float* U0, const float* U1) {
+    constexpr int TILES = decltype(tiles)::value;
+    const int second = 8 * (U1 != nullptr ? ub + 1 : ub);
+    uint32_t held[G::HOLD ? TILES : 1][2][QP];
+    auto fragments = [&](uint32_t (&x)[2][QP], int nt) {
+      x_pieces(x[0], nt, 8 * ub, ub != ua);
+      x_pieces(x[1], nt, second, true);
+    };
+    if (G::HOLD) {
 #pragma unroll
-          for (int i = 0; i < SP; ++i) a[i][2] = a[i][3] = 0u;
-        }
-        const float* scale = sX + (8 * ua + mi) * N + t2;
+      for (int nt = 0; nt < TILES; ++nt) fragments(held[G::HOLD ? nt : 0], nt);
+    }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if (8 * nt < n) {
-            uint32_t b0[QP], b1[QP];
-            x_pieces(b0, 8 * nt + g, 8 * ub + t2);
-            x_pieces(b1, 8 * nt + g, 8 * (count == 2 ? ub + 1 : ub) + t2);
+    for (int r = 0; r < RI; ++r) {
+      const int at = (8 * (kg * RI + r) + t2) * LDS + column;
+      uint32_t a[SP][4];
+      s_pieces(a, 0, U0 + at);
+      if (U1 != nullptr) {
+        s_pieces(a, 1, U1 + at);
+      } else {   // without a second unit its terms are zeros
 #pragma unroll
-            for (int p = 0; p < QP; ++p) {
-              if (ub != ua) b0[p] = twice(b0[p]);
-              b1[p] = twice(b1[p]);
-            }
-            float c[4] = {};
-            products(c, a, b0, b1);
-            const float2 x = *reinterpret_cast<const float2*>(scale + 8 * nt);
-            acc[nt][0] = fmaf(x.x, c[0], acc[nt][0]);
-            acc[nt][1] = fmaf(x.y, c[1], acc[nt][1]);
-            acc[nt][2] = fmaf(x.x, c[2], acc[nt][2]);
-            acc[nt][3] = fmaf(x.y, c[3], acc[nt][3]);
-          }
+        for (int k = 0; k < SP; ++k) a[k][2] = a[k][3] = 0u;
       }
-      if (step % G::WARPS == warp) {
-        // the last column: rows of the product are the eight m instead
-        uint32_t a[SP][4];
-        s_pieces(a, 0, U + (8 * g + t2) * LDS + D, LDS);
-        if (count == 2) s_pieces(a, 2, U + G::UNIT + (8 * g + t2) * LDS + D, LDS);
+      const float* scale = sX + (8 * ua + kg * RI + r) * N + t2;
 #pragma unroll
-        for (int i = 0; i < SP; ++i) {
-          a[i][1] = a[i][3] = 0u;
-          if (count != 2) a[i][2] = 0u;
-        }
-        const float* scale = sX + (8 * ua + g) * N + t2;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if (8 * nt < n) {
-            uint32_t b0[QP], b1[QP];
-            x_pieces(b0, 8 * nt + g, 8 * ub + t2);
-            x_pieces(b1, 8 * nt + g, 8 * (count == 2 ? ub + 1 : ub) + t2);
-#pragma unroll
-            for (int p = 0; p < QP; ++p) {
-              if (ub != ua) b0[p] = twice(b0[p]);
-              b1[p] = twice(b1[p]);
-            }
-            float c[4] = {};
-            products(c, a, b0, b1);
-            const float2 x = *reinterpret_cast<const float2*>(scale + 8 * nt);
-            den[nt][0] = fmaf(x.x, c[0], den[nt][0]);
-            den[nt][1] = fmaf(x.y, c[1], den[nt][1]);
-          }
+      for (int nt = 0; nt < TILES; ++nt) {
+        if (!G::HOLD) fragments(held[0], nt);
+        const float2 xm = *reinterpret_cast<const float2*>(scale + 8 * nt);
+        float c[4];
+        products(c, a, held[G::HOLD ? nt : 0]);
+        fma2(acc[nt][0], acc[nt][1], xm, c[0], c[1]);
+        fma2(acc[nt][2], acc[nt][3], xm, c[2], c[3]);
       }
-      u += count, ub += count;
-      if (ub >= NB) ++ua, ub = ua;
-    } else {
-      // the linear rows: x_m S[m] and the constant's row.  What was summed so far takes its weight.
-      const float c1 = P.a1 * P.inv_t, c2 = P.a2 * P.inv_t * P.inv_t;
+    }
+    if (step % G::WARPS == warp) {   // the last column: the rows of its product are the eight m instead
+      const int at = (8 * g + t2) * LDS + D;
+      uint32_t a[SP][4] = {};
+      last_pieces(a, 0, U0 + at);
+      if (U1 != nullptr) last_pieces(a, 1, U1 + at);
+      const float* scale = sX + (8 * ua + g) * N + t2;
+#pragma unroll
+      for (int nt = 0; nt < TILES; ++nt) {
+        if (!G::HOLD) fragments(held[0], nt);
+        const float2 xm = *reinterpret_cast<const float2*>(scale + 8 * nt);
+        float c[4];
+        products(c, a, held[G::HOLD ? nt : 0]);
+        den[nt][0] = fmaf(xm.x, c[0], den[nt][0]);
+        den[nt][1] = fmaf(xm.y, c[1], den[nt][1]);
+      }
+    }
+  };
+  int done = 0;   // units
+  auto unit = [&](int i) -> const float* {
+    wait(&full[i % SLOTS], (uint32_t)(i / SLOTS) & 1u, 210, abort_flag);
+    return reinterpret_cast<const float*>(smem + (i % SLOTS) * G::SLOT);
+  };
+  // the last warp that is done with a step asks for the units that take its slots
+  auto release = [&](int i, int units) {
+    if (u_first + i + SLOTS >= u_end) return;
+    if (count_up(&through[i % SLOTS]) == G::WARPS - 1 && *abort_flag == 0) {
+      through[i % SLOTS] = 0;   // seen by whoever finds the next copy arrived
+      load(i + SLOTS);
+      if (units == 2 && u_first + i + 1 + SLOTS < u_end) load(i + 1 + SLOTS);
+    }
+  };
+  while (u_first + done < min(u_end, npairs)) {
+    const bool pair = ub + 1 < NB && u_first + done + 1 < u_end;
+    const float* U0 = unit(done);
+    const float* U1 = pair ? unit(done + 1) : nullptr;
+    const int tiles = (n + 7) / 8;
+    if (NT <= 2 || tiles > 3 * NT / 4) pair_step(std::integral_constant<int, NT>{}, U0, U1);
+    else if (tiles > NT / 2) pair_step(std::integral_constant<int, NT <= 2 ? NT : 3 * NT / 4>{}, U0, U1);
+    else pair_step(std::integral_constant<int, NT <= 2 ? NT : NT / 2>{}, U0, U1);
+    __syncwarp();
+    if (lane == 0) release(done, pair ? 2 : 1);
+    done += pair ? 2 : 1, ub += pair ? 2 : 1, ++step;
+    if (ub >= NB) ++ua, ub = ua;
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {   // the weight of all pairs
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[nt][j] *= c2;
+    den[nt][0] *= c2, den[nt][1] *= c2;
+  }
+  if (u_end > npairs) {
+    // the linear rows, x_m S[m], 16 of them a warp, and the constant's row
+    const float* U = unit(done);
+    for (int ks = kg; ks < D / 16; ks += KG) {
+      uint32_t a[SP][4], al[SP][4] = {};
+      const float* rows = U + (16 * ks + t2) * LDS;
+      s_pieces(a, 0, rows + column);
+      s_pieces(a, 1, rows + 8 * LDS + column);
+      if (g == 0 && warp % G::CG == 0) {   // the last column, as a product of one row
+        last_pieces(al, 0, rows + D);
+        last_pieces(al, 1, rows + 8 * LDS + D);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        if (8 * nt < n) {
+          uint32_t x[2][QP];
+          x_pieces(x[0], nt, 16 * ks, false);
+          x_pieces(x[1], nt, 16 * ks + 8, false);
+          float c[4];
+          products(c, a, x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[nt][j] = fmaf(c1, c[j], acc[nt][j]);
+          products(c, al, x);
+          den[nt][0] = fmaf(c1, c[0], den[nt][0]);
+          den[nt][1] = fmaf(c1, c[1], den[nt][1]);
+        }
+    }
+    if (kg == KG - 1) {
+      const float2 ones = *reinterpret_cast<const float2*>(U + D * LDS + column);
+      const float last = g == 0 && warp % G::CG == 0 ? P.a0 * U[D * LDS + D] : 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] *= c2;
-        den[nt][0] *= c2, den[nt][1] *= c2;
+        acc[nt][0] = fmaf(P.a0, ones.x, acc[nt][0]), acc[nt][1] = fmaf(P.a0, ones.x, acc[nt][1]);
+        acc[nt][2] = fmaf(P.a0, ones.y, acc[nt][2]), acc[nt][3] = fmaf(P.a0, ones.y, acc[nt][3]);
+        den[nt][0] += last, den[nt][1] += last;
       }
-      for (int ks = kg; ks < D / 16; ks += G::KG) {
-        const float* row = U + (16 * ks + t2) * LDS + 16 * mt + g;
-        uint32_t a[SP][4], ad[SP][4];
-        s_pieces(a, 0, row, LDS);
-        s_pieces(a, 1, row + 8, LDS);
-        s_pieces(a, 2, row + 8 * LDS, LDS);
-        s_pieces(a, 3, row + 8 * LDS + 8, LDS);
-        if (mt == 0) {   // and the last column, as a product of one row
-          const float* last = U + (16 * ks + t2) * LDS + D;
-          s_pieces(ad, 0, last, LDS);
-          s_pieces(ad, 2, last + 8 * LDS, LDS);
-#pragma unroll
-          for (int i = 0; i < SP; ++i) {
-            ad[i][1] = ad[i][3] = 0u;
-            if (g != 0) ad[i][0] = ad[i][2] = 0u;
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if (8 * nt < n) {
-            uint32_t b0[QP], b1[QP];
-            x_pieces(b0, 8 * nt + g, 16 * ks + t2);
-            x_pieces(b1, 8 * nt + g, 16 * ks + 8 + t2);
-            float c[4] = {};
-            products(c, a, b0, b1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[nt][i] = fmaf(c1, c[i], acc[nt][i]);
-            if (mt == 0) {
-              float cd[4] = {};
-              products(cd, ad, b0, b1);
-              den[nt][0] = fmaf(c1, cd[0], den[nt][0]);
-              den[nt][1] = fmaf(c1, cd[1], den[nt][1]);
-            }
-          }
-      }
-      if (kg == G::KG - 1) {
-        const float* ones = U + D * LDS;
-        const float s0 = P.a0 * ones[16 * mt + g], s1 = P.a0 * ones[16 * mt + g + 8], sd = mt == 0 && g == 0 ? P.a0 * ones[D] : 0.f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          acc[nt][0] += s0, acc[nt][1] += s0, acc[nt][2] += s1, acc[nt][3] += s1;
-          den[nt][0] += sd, den[nt][1] += sd;
-        }
-      }
-      u += 1;
-    }
-    slot = slot + 1 == G::SLOTS ? 0 : slot + 1;
-    ++step;
-  }
-  if (u_end <= npairs) {   // the linear rows are another block's: the weight here
-    const float c2 = P.a2 * P.inv_t * P.inv_t;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[nt][i] *= c2;
-      den[nt][0] *= c2, den[nt][1] *= c2;
     }
   }
-  copies_wait<0>();
-  __syncthreads();
-  // ---- partial sums meet: warps of a block, then blocks of the cluster, both in a fixed order ----------------------------------
-  float* red = slots;                          // [KG][N][LDS]
-  float* last = slots + G::KG * N * LDS;       // [WARPS][N]
+  __syncthreads();   // nobody reads values and weights any more
+  if (tid == 0 && *abort_flag != 0)   // leave only after the copies in flight
+    for (int i = 0; i < SLOTS; ++i)
+      if (issued[i] > 0) mbar_wait_bounded(&full[i], (uint32_t)(issued[i] - 1) & 1u, WAIT_CYCLES);
+  // ---- partial sums meet, the warps' and the cluster's blocks', in a fixed order ------------------------------------------------
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    float* at = red + (kg * N + 8 * nt + t2) * LDS + 16 * mt + g;
-    at[0] = acc[nt][0], at[LDS] = acc[nt][1], at[8] = acc[nt][2], at[LDS + 8] = acc[nt][3];
+  for (int nt = 0; nt < NT; ++nt)
+    if (8 * nt < n) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float d = den[nt][i];
-      d += __shfl_xor_sync(0xffffffffu, d, 4);
-      d += __shfl_xor_sync(0xffffffffu, d, 8);
-      d += __shfl_xor_sync(0xffffffffu, d, 16);
-      if (g == 0) last[warp * N + 8 * nt + t2 + i] = d;
-    }
-  }
-  __syncthreads();
-  for (int idx = tid; idx < n * C4; idx += THREADS) {
-    const int i = idx / C4, c = 4 * (idx - i * C4);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < D) {
-#pragma unroll
-      for (int w = 0; w < G::KG; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(red + (w * N + i) * LDS + c);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      for (int e = 0; e < 2; ++e) {
+        float* at = part + (kg * N + 8 * nt + t2 + e) * LDS;
+        *reinterpret_cast<float2*>(at + column) = make_float2(acc[nt][e], acc[nt][2 + e]);
+        float d = den[nt][e];
+        d += __shfl_xor_sync(0xffffffffu, d, 4);
+        d += __shfl_xor_sync(0xffffffffu, d, 8);
+        d += __shfl_xor_sync(0xffffffffu, d, 16);
+        if (g < (G::CG == 4 ? 1 : 4 / G::CG)) at[D + warp % G::CG + G::CG * g] = g == 0 ? d : 0.f;   // four parts, added up at the end
       }
-    } else {
-#pragma unroll
-      for (int w = 0; w < G::WARPS; ++w) x.x += last[w * N + i];
     }
-    *reinterpret_cast<float4*>(red + i * LDS + c) = x;   // nobody else reads or writes these
-  }
-  cluster.sync();
+  meet();
   for (int idx = tid; idx < mine * C4; idx += THREADS) {
     const int i = idx / C4, c = 4 * (idx - i * C4);
     float4 x = *reinterpret_cast<const float4*>(sT + i * LDS + c);
     for (int r = 0; r < CL; ++r) {
-      const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(red, r) + (i0 + i) * LDS + c);
-      x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      const float* sums = (CL > 1 ? cluster.map_shared_rank(part, r) : part) + (i0 + i) * LDS + c;
+#pragma unroll
+      for (int w = 0; w < KG; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(sums + w * N * LDS);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      }
     }
     *reinterpret_cast<float4*>(sT + i * LDS + c) = x;
   }
-  cluster.sync();   // (also: nobody's shared memory is read any more)
+  meet();   // (also: nobody's sums are read any more)
   T* o = const_cast<T*>(head_base<T>(P.o, head, P.heads));
   for (int idx = tid; idx < mine * (D / 4); idx += THREADS) {
     const int i = idx / (D / 4), c = 4 * (idx - i * (D / 4));
-    const float sum = sT[i * LDS + D];
+    const float4 last = *reinterpret_cast<const float4*>(sT + i * LDS + D);
+    const float total = (last.x + last.y) + (last.z + last.w);
     const float4 x = *reinterpret_cast<const float4*>(sT + i * LDS + c);
-    store4v(o + (i0 + i) * P.o.sn + c, P.aligned, x.x / sum, x.y / sum, x.z / sum, x.w / sum);
-    if (c == 0 && P.g.ptr != nullptr) const_cast<float*>(head_base<float>(P.g, head, P.heads))[(i0 + i) * P.g.sn] = sum;
+    store4v(o + (i0 + i) * P.o.sn + c, P.aligned, x.x / total, x.y / total, x.z / total, x.w / total);
+    if (c == 0 && P.g.ptr != nullptr) const_cast<float*>(head_base<float>(P.g, head, P.heads))[(i0 + i) * P.g.sn] = total;
   }
 }
 
@@ -564,8 +674,10 @@ static cudaError_t launch_attention(const TreeParams& P, int bh, cudaStream_t st
   using G = TreeGeo<T, D, NT>;
   cudaError_t e = allow_bytes<attention_kernel<T, D, NT>>(G::BYTES);
   if (e != cudaSuccess) return e;
+  // A head is divided among blocks of a cluster as far as all blocks then still run at once and each has two units or more.
+  const int units = (P.order == 2 ? Geo<D>::NPAIRS : 0) + 1;
   int cl = 1;
-  while (cl < 8 && (long long)cl * bh < 4 * sm_count()) cl *= 2;
+  while (cl < 8 && 2LL * cl * bh <= (long long)G::BLOCKS * sm_count() && 4 * cl <= units + 1) cl *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cl, bh);
   cfg.blockDim = dim3(G::THREADS);
@@ -638,6 +750,26 @@ static TreeParams params(const fastmax_problem* pb, const fastmax_pages& cache, 
 static View view(const fastmax_tensor& t) { return View{t.ptr, t.stride_b, t.stride_h, t.stride_n}; }
 
 }  // namespace tree
+
+int tree_status(int* out) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, tree::g_status, sizeof(int), 0, cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) return report_cuda_error(e);
+  if (*out != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(tree::g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice);
+  }
+  return FASTMAX_OK;
+}
+int tree_wait_histogram(int* out, int n) {
+  int h[256];
+  cudaError_t e = cudaMemcpyFromSymbol(h, tree::g_wait_hist, sizeof(h), 0, cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) return report_cuda_error(e);
+  for (int i = 0; i < n && i < 256; ++i) out[i] += h[i];
+  static const int zeros[256] = {0};
+  cudaMemcpyToSymbol(tree::g_wait_hist, zeros, sizeof(zeros), 0, cudaMemcpyHostToDevice);
+  return FASTMAX_OK;
+}
+
 }  // namespace fm
 
 extern "C" int32_t fastmax_tree_attention(const fastmax_problem* pb, const fastmax_tree_args* a, void* cuda_stream) {
