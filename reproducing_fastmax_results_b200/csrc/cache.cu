@@ -72,19 +72,21 @@ arrange_plan_kernel(int* table, const int* sources, int places, int pages, int* 
   __syncthreads();
   grid_wait();
   grid_trigger();
-  for (int i = tid; i < places; i += PLAN_THREADS) {
-    const int j = sources[i];
-    int held = -1;
-    if (j >= 0 && j < places) {
-      held = table[j];
-      if (held < 0 || held >= pages) held = -1;
-      if (held >= 0) atomicMin(&first[held], i);
-    } else if (j == -2) {
-      held = -2;
-    } else if (j != -1) {
-      atomicAdd(&wrong, 1);
+  constexpr int BATCH = 4;   // places of a thread whose loads are under way together
+  for (int i0 = tid; i0 < places; i0 += BATCH * PLAN_THREADS) {
+    int j[BATCH], held[BATCH];
+#pragma unroll
+    for (int t = 0; t < BATCH; ++t) j[t] = i0 + t * PLAN_THREADS < places ? sources[i0 + t * PLAN_THREADS] : -1;
+#pragma unroll
+    for (int t = 0; t < BATCH; ++t) held[t] = j[t] >= 0 && j[t] < places ? table[j[t]] : -1;
+#pragma unroll
+    for (int t = 0; t < BATCH; ++t) {
+      const int i = i0 + t * PLAN_THREADS;
+      if (held[t] < 0 || held[t] >= pages) held[t] = j[t] == -2 ? -2 : -1;
+      if (j[t] < -2 || j[t] >= places) atomicAdd(&wrong, 1);
+      if (held[t] >= 0) atomicMin(&first[held[t]], i);
+      if (i < places) L.held[i] = held[t];   // read again by this thread alone
     }
-    L.held[i] = held;   // read again by this thread alone
   }
   __syncthreads();   // from here on nobody reads the table any more
   int nfree = 0;
@@ -96,9 +98,11 @@ arrange_plan_kernel(int* table, const int* sources, int places, int pages, int* 
   }
   __syncthreads();
   int nwant = 0;
+  int ahead = tid < places ? L.held[tid] : -1;
   for (int i0 = 0; i0 < places; i0 += PLAN_THREADS) {
     const int i = i0 + tid;
-    const int held = i < places ? L.held[i] : -1;
+    const int held = ahead;
+    ahead = i + PLAN_THREADS < places ? L.held[i + PLAN_THREADS] : -1;
     const bool keeps = held >= 0 && first[held] == i;
     const bool wants = held == -2 || (held >= 0 && !keeps);
     const int r = block_rank(wants, nwant, sums);
@@ -185,43 +189,63 @@ struct CopyParams {
 };
 
 constexpr int COPY_THREADS = 256;
-constexpr int COPY_UNROLL = 4;
-constexpr int COPY_CHUNK = COPY_THREADS * COPY_UNROLL;   // float4 that a block has in flight: 16 KB
+constexpr int COPY_UNROLL = 2;
+constexpr int COPY_CHUNK = COPY_THREADS * COPY_UNROLL;   // float4 of a step: 8 KB
+constexpr int COPY_BLOCKS = 4;                           // to an SM
+// 64 KB in flight an SM.  GB/s at 760 MB read and written (a copy of one tensor by PyTorch: 6440), steps of KB x blocks to an SM: 8 x 4
+// 6390, 8 x 3 5850, 8 x 5 5850, 16 x 2 6220, 16 x 4 5870, 32 x 1 5990, 32 x 2 5910, 4 x 8 6050; streaming loads too 6290, ordinary stores 6160.
 
-__global__ void __launch_bounds__(COPY_THREADS)
+// A block's steps are gridDim.x chunks apart; the next step's loads are in flight while one is stored.
+__global__ void __launch_bounds__(COPY_THREADS, COPY_BLOCKS)
 pages_copy_kernel(const CopyParams P) {
   grid_wait();
   grid_trigger();
   const int count = P.count_at != nullptr ? *P.count_at : P.count;
   const long long chunks = (P.page + COPY_CHUNK - 1) / COPY_CHUNK;
-  for (long long w = blockIdx.x; w < chunks * count; w += gridDim.x) {
-    const int i = (int)(w / chunks);
-    const long long at = (w - i * chunks) * COPY_CHUNK + threadIdx.x;
+  struct Step {
+    float4 x[COPY_UNROLL];
+    float4* to;     // NULL: nothing to store
+    int quads;      // of this thread's: the first of them lies at the thread's number
+  };
+  int i = (int)(blockIdx.x / chunks);
+  long long c = blockIdx.x - i * chunks;
+  auto fetch = [&](Step& s) {
+    s.to = nullptr;
+    if (i >= count) return;
     const int from = P.src_index != nullptr ? P.src_index[i] : i;
     const int to = P.dst_index != nullptr ? P.dst_index[i] : i;
-    if (to < 0 || to >= P.dst_pages) continue;
-    float4 x[COPY_UNROLL];
-    if (from >= 0 && from < P.src_pages) {
-      const float4* s = P.src + from * P.src_stride + at;
+    const bool known = from >= 0 && from < P.src_pages;
+    const long long at = c * COPY_CHUNK;
+    s.quads = (int)(P.page - at < COPY_CHUNK ? P.page - at : COPY_CHUNK);
+    if (to >= 0 && to < P.dst_pages && (known || P.clear)) s.to = P.dst + to * P.dst_stride + at + threadIdx.x;
+    const float4* src = P.src + from * P.src_stride + at + threadIdx.x;
 #pragma unroll
-      for (int j = 0; j < COPY_UNROLL; ++j)
-        if (at + j * COPY_THREADS < P.page) x[j] = __ldcs(s + j * COPY_THREADS);
-    } else if (P.clear) {
-#pragma unroll
-      for (int j = 0; j < COPY_UNROLL; ++j) x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    } else {
-      continue;
+    for (int j = 0; j < COPY_UNROLL; ++j) {
+      s.x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (known && s.to != nullptr && (int)threadIdx.x + j * COPY_THREADS < s.quads) s.x[j] = src[j * COPY_THREADS];
     }
-    float4* d = P.dst + to * P.dst_stride + at;
+    c += gridDim.x;
+    while (c >= chunks) c -= chunks, ++i;
+  };
+  auto put = [&](const Step& s) {
+    if (s.to == nullptr) return;
 #pragma unroll
     for (int j = 0; j < COPY_UNROLL; ++j)
-      if (at + j * COPY_THREADS < P.page) __stcs(d + j * COPY_THREADS, x[j]);
+      if ((int)threadIdx.x + j * COPY_THREADS < s.quads) __stcs(s.to + j * COPY_THREADS, s.x[j]);
+  };
+  Step a, b;
+  fetch(a);
+  while (i < count) {
+    fetch(b);
+    put(a);
+    a = b;
   }
+  put(a);
 }
 
 static cudaError_t launch_copy(const CopyParams& P, int most, cudaStream_t st) {
   const long long chunks = (P.page + COPY_CHUNK - 1) / COPY_CHUNK;
-  const long long room = 8LL * sm_count();   // resident blocks; each goes on to the next chunk
+  const long long room = (long long)COPY_BLOCKS * sm_count();
   const long long blocks = most * chunks < room ? most * chunks : room;
   LaunchScope ls(KK_CACHE_COPY, st);
   return launch_after(pages_copy_kernel, dim3((unsigned)blocks), COPY_THREADS, 0, st, P);

@@ -624,36 +624,122 @@ attention_kernel(const TreeParams P) {
   }
 }
 
-template <typename T, int D, int ORDER>
-__global__ void accept_kernel(const TreeParams P) {
-  using G = Geo<D>;
+// ---- taking a path ---------------------------------------------------------------------------------------------------------
+// S[(m, n)][:] += sum over the path of k_m (k_n [v | 1]): every float of the state is read and written once.  A thread has one float4 column of four
+// rows of a unit, (m .. m + 3, n), and the next unit's four in flight meanwhile; k_n v is made once for the four.
+template <int D>
+struct AcceptGeo {
+  static constexpr int C4 = (D + 4) / 4;
+  static constexpr int THREADS = 16 * C4;              // 64 rows of a unit, four to a thread
+  static constexpr int LV = D + 4;
+  static int bytes(int nodes) { return nodes * (D + LV) * 4 + nodes * 8; }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(AcceptGeo<D>::THREADS)
+accept_kernel(const TreeParams P, int units_each) {
+  using G = AcceptGeo<D>;
+  constexpr int C4 = G::C4, LV = G::LV, NB = D / 8, THREADS = G::THREADS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* sK = reinterpret_cast<float*>(smem);              // [nodes][D]: keys of the path, from the root down
+  float* sV = sK + P.nodes * D;                            // [nodes][LV]: [v | 1 0 0 0]
+  int* path = reinterpret_cast<int*>(sV + P.nodes * LV);   // [nodes]
+  int* up = path + P.nodes;                                // [nodes]
+  __shared__ int length;
+  const int tid = threadIdx.x, head = blockIdx.y, b = head / P.heads;
+  const int npairs = P.order == 2 ? Geo<D>::NPAIRS : 0;
+  const int u0 = blockIdx.x * units_each, u1 = min(u0 + units_each, npairs + 1);
   grid_wait();
   grid_trigger();
-  const int b = blockIdx.y / P.heads, h = blockIdx.y - b * P.heads;
-  float* S = head_state(P, b, h, D);
-  if (S == nullptr || P.ends[b] < 0 || P.ends[b] >= P.nodes) return;
-  const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int r = (int)(at / (D + 4)), c = (int)(at - (long long)r * (D + 4));
-  if (r >= P.rows || c > D) return;
-  int path[FASTMAX_TREE_NODES], n = 0;
-  for (int j = P.ends[b]; j >= 0; j = parent_of(P, b, j)) path[n++] = j;
-  float s = S[at];
-  while (n > 0) {
-    const int j = path[--n];
-    const T* k = head_base<T>(P.k, blockIdx.y, P.heads) + j * P.k.sn;
-    const T* v = head_base<T>(P.v, blockIdx.y, P.heads) + j * P.v.sn;
-    float f = 1.f;
-    if (ORDER == 2 && r < 64 * G::NPAIRS) {
-      int x, y;
-      pair_decode(r >> 6, G::NB, x, y);
-      f = load1(k + 8 * x + ((r & 63) >> 3)) * load1(k + 8 * y + (r & 7));
+  const int last = P.ends[b];
+  float* S = head_state(P, b, head - b * P.heads, D);
+  if (S == nullptr || last < 0 || last >= P.nodes) return;
+
+  const int c4 = tid % C4, rg = tid / C4;
+  const int n8 = rg & 7, m8 = 4 * (rg >> 3);               // of a pair of blocks: rows (m8 .. m8 + 3, n8)
+  auto row_of = [&](int u, int j) { return u < npairs ? 64 * u + 8 * (m8 + j) + n8 : 64 * npairs + rg + 16 * j; };
+  auto there = [&](int u, int j) { return u < npairs || rg + 16 * j < D; };
+  float4* base = reinterpret_cast<float4*>(S) + c4;
+  float4 next[4], ones = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto fetch = [&](int u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (there(u, j)) next[j] = __ldcs(base + (long long)row_of(u, j) * C4);
+    if (u == npairs && rg == 0) ones = __ldcs(base + (long long)(64 * npairs + D) * C4);   // the constant's row
+  };
+  fetch(u0);
+  if (P.parents != nullptr)
+    for (int i = tid; i <= last; i += THREADS) up[i] = parent_of(P, b, i);
+  __syncthreads();
+  if (tid == 0) {
+    int n = 0;
+    if (P.parents == nullptr) {
+      n = last + 1;
     } else {
-      const int m = r - (ORDER == 2 ? 64 * G::NPAIRS : 0);
-      if (m < D) f = load1(k + m);
+      for (int i = last; i >= 0; i = up[i]) path[n++] = i;
     }
-    s = fmaf(f, c < D ? load1(v + c) : 1.f, s);
+    length = n;
   }
-  S[at] = s;
+  __syncthreads();
+  const int n = length;
+  {
+    const T* k = head_base<T>(P.k, head, P.heads);
+    const T* v = head_base<T>(P.v, head, P.heads);
+    for (int idx = tid; idx < n * C4; idx += THREADS) {
+      const int i = idx / C4, c = 4 * (idx - i * C4);
+      const int node = P.parents == nullptr ? i : path[n - 1 - i];
+      float x[4], y[4] = {1.f, 0.f, 0.f, 0.f};
+      if (c < D) {
+        Raw4<T> rk, rv;
+        rk.load(k + node * P.k.sn + c, P.aligned);
+        rv.load(v + node * P.v.sn + c, P.aligned);
+        rk.get(true, x);
+        rv.get(true, y);
+        *reinterpret_cast<float4*>(sK + i * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+      }
+      *reinterpret_cast<float4*>(sV + i * LV + c) = make_float4(y[0], y[1], y[2], y[3]);
+    }
+  }
+  __syncthreads();
+  int ua = 0, ub = 0;
+  if (u0 < npairs) pair_decode(u0, NB, ua, ub);
+  for (int u = u0; u < u1; ++u) {
+    float4 s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = next[j];
+    if (u + 1 < u1) fetch(u + 1);
+    if (u < npairs) {
+      const float* km = sK + 8 * ua + m8;
+      const float* kn = sK + 8 * ub + n8;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float4 m = *reinterpret_cast<const float4*>(km + i * D);
+        const float4 y = *reinterpret_cast<const float4*>(sV + i * LV + 4 * c4);
+        const float x = kn[i * D];
+        const float4 w = make_float4(x * y.x, x * y.y, x * y.z, x * y.w);
+        fma2(s[0].x, s[0].y, make_float2(m.x, m.x), w.x, w.y), fma2(s[0].z, s[0].w, make_float2(m.x, m.x), w.z, w.w);
+        fma2(s[1].x, s[1].y, make_float2(m.y, m.y), w.x, w.y), fma2(s[1].z, s[1].w, make_float2(m.y, m.y), w.z, w.w);
+        fma2(s[2].x, s[2].y, make_float2(m.z, m.z), w.x, w.y), fma2(s[2].z, s[2].w, make_float2(m.z, m.z), w.z, w.w);
+        fma2(s[3].x, s[3].y, make_float2(m.w, m.w), w.x, w.y), fma2(s[3].z, s[3].w, make_float2(m.w, m.w), w.z, w.w);
+      }
+      if (++ub == NB) ub = ++ua;
+    } else {
+      for (int i = 0; i < n; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(sV + i * LV + 4 * c4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (there(u, j)) {
+            const float x = sK[i * D + rg + 16 * j];
+            s[j].x = fmaf(x, y.x, s[j].x), s[j].y = fmaf(x, y.y, s[j].y), s[j].z = fmaf(x, y.z, s[j].z), s[j].w = fmaf(x, y.w, s[j].w);
+          }
+        ones.x += y.x, ones.y += y.y, ones.z += y.z, ones.w += y.w;
+      }
+      if (rg == 0) __stcs(base + (long long)(64 * npairs + D) * C4, ones);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (there(u, j)) __stcs(base + (long long)row_of(u, j) * C4, s[j]);
+  }
 }
 
 // Dynamic shared memory beyond 48 KB has to be allowed once per device and kernel.
@@ -694,11 +780,18 @@ static cudaError_t launch_attention(const TreeParams& P, int bh, cudaStream_t st
   return launched(cudaLaunchKernelEx(&cfg, attention_kernel<T, D, NT>, P));
 }
 template <typename T, int D>
+static cudaError_t launch_accept(const TreeParams& P, int bh, cudaStream_t st) {
+  const int units = (P.order == 2 ? Geo<D>::NPAIRS : 0) + 1;
+  // Four units a block where the launch still has some blocks for every SM, so that a unit's loads cover the one before it; fewer where
+  // it would not.  us with 1 / 2 / 4 / 8 units, paths of 4 or 5: d = 64, 8 heads 4.4 / 4.4 / 5.6 / 8.3, 512 heads 126 / 106 / 101 / 106; d = 16,
+  // 512 heads 5.7 / 5.4 / 6.2 / 6.2.
+  int each = 4;
+  while (each > 1 && (long long)((units + each - 1) / each) * bh < 4LL * sm_count()) each /= 2;
+  return launch_after(accept_kernel<T, D>, dim3((unsigned)((units + each - 1) / each), (unsigned)bh), AcceptGeo<D>::THREADS, AcceptGeo<D>::bytes(P.nodes), st, P, each);
+}
+template <typename T, int D>
 static cudaError_t launch(bool attend, const TreeParams& P, int bh, cudaStream_t st) {
-  if (!attend) {
-    const dim3 grid((unsigned)((P.rows * (D + 4) + 255) / 256), (unsigned)bh);
-    return P.order == 2 ? launch_after(accept_kernel<T, D, 2>, grid, 256, 0, st, P) : launch_after(accept_kernel<T, D, 1>, grid, 256, 0, st, P);
-  }
+  if (!attend) return launch_accept<T, D>(P, bh, st);
   return P.nodes <= 8    ? launch_attention<T, D, 1>(P, bh, st)
          : P.nodes <= 16 ? launch_attention<T, D, 2>(P, bh, st)
          : P.nodes <= 32 ? launch_attention<T, D, 4>(P, bh, st)
@@ -800,6 +893,7 @@ extern "C" int32_t fastmax_tree_accept(const fastmax_problem* pb, const fastmax_
   if (const int rc = check_pages(pb, a->cache)) return rc;
   tree::TreeParams P = tree::params(pb, a->cache, a->parents, a->parents_stride, a->last);
   P.k = tree::view(a->k), P.v = tree::view(a->v);
+  P.aligned = tree::rows_aligned(a->k, pb->dtype) && tree::rows_aligned(a->v, pb->dtype);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   cudaError_t e;
   {
