@@ -38,6 +38,7 @@ class FastmaxCache:
         self.a0, self.a1, self.a2 = float(a0), float(a1), float(a2)
         self.state = _lib.new_state(self.pages * self.layers, self.heads, self.d, self.p, device).unflatten(0, (self.pages, self.layers))
         self.table = torch.full((self.places,), -1, dtype=torch.int32, device=device)
+        self._states = self.state.unbind(1)   # a layer's (pages, heads, rows, d + 4)
 
     # ---- pages -----------------------------------------------------------------------------------------------------------
     def arrange(self, sources):
@@ -73,12 +74,7 @@ class FastmaxCache:
     def _layer(self, layer):
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer: 0 to {self.layers - 1} expected, got {layer}")
-        return self.state[:, layer]
-
-    def _check(self, t, name, dims):
-        shape = tuple(t.shape)
-        if t.dim() not in dims or shape[:2] != (self.places, self.heads) or shape[-1] != self.d:
-            raise ValueError(f"{name}: expected ({self.places}, {self.heads}, ..., {self.d}), got {shape}")
+        return self._states[layer]
 
     def prefill(self, q, k, v, places, layer=0, continues=False):
         """Causal attention of prompts, (len(places), h, n, d), whose sequences are in `places` (different numbers on the host; they have
@@ -102,20 +98,14 @@ class FastmaxCache:
     def step(self, q, k, v, layer=0, out=None):
         """One new token per place: q, k, v are (places, h, d) or (places, h, 1, d).  Returns o shaped like q; rows of places without a
         page stay as they are in `out`, zero without one."""
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            self._check(t, name, (3, 4))
         return _ext().decode_step_paged(q, k, v, self._layer(layer), self.table, self.inv_temperature, self.a0, self.a1, self.a2, self.p, out)
 
     def verify(self, q, k, v, parents=None, lengths=None, layer=0, out=None):
         """Attention of drafted tokens, (places, h, n, d) with n <= 64, as in FastmaxDecoder.verify.  Rows of places without a page and rows
         behind a place's nodes stay as they are in `out`, zero without one."""
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            self._check(t, name, (4,))
         return _ext().tree_attention(q, k, v, self._layer(layer), self.table, tree_parents(parents, q), per_sequence(lengths, q, "lengths", 0, q.shape[2]),
                                      self.inv_temperature, self.a0, self.a1, self.a2, self.p, out)
 
     def accept(self, k, v, last, parents=None, layer=0):
         """Takes the path to node last[i] into the state of place i, as in FastmaxDecoder.accept.  Every layer takes its own k and v."""
-        for t, name in ((k, "k"), (v, "v")):
-            self._check(t, name, (4,))
         _ext().tree_accept(k, v, self._layer(layer), per_sequence(last, k, "last", -1, k.shape[2] - 1), self.table, tree_parents(parents, k), self.p)

@@ -533,109 +533,106 @@ torch::Tensor decode_step(torch::Tensor q, torch::Tensor k, torch::Tensor v, tor
 using maybe = c10::optional<torch::Tensor>;
 bool given(const maybe& t) { return t.has_value() && t->defined(); }
 
+// Shapes are checked here, before anything else and as ValueError: the Python classes pass their arguments straight on.
 // state: float32 (pages, heads, rows, ld), pages any distance apart (a layer of a cache); table: int32 (batch,) or none
 fastmax_pages pages_of(const torch::Tensor& state, const maybe& table, const fastmax_problem& pb) {
-  CHECK_CUDA(state);
   const int64_t rows = fastmax_state_rows(pb.d, pb.order), ld = fastmax_state_ld(pb.d);
-  TORCH_CHECK(state.scalar_type() == torch::kFloat32 && state.dim() == 4 && state.size(1) == pb.heads && state.size(2) == rows && state.size(3) == ld &&
-                  state.stride(3) == 1 && state.stride(2) == ld && (pb.heads == 1 || state.stride(1) == rows * ld),
+  TORCH_CHECK(state.scalar_type() == torch::kFloat32 && state.stride(3) == 1 && state.stride(2) == ld && state.size(2) == rows && state.size(3) == ld &&
+                  (pb.heads == 1 || state.stride(1) == rows * ld) && state.size(0) <= INT32_MAX,
               "state must be float32 (pages, ", pb.heads, ", ", rows, ", ", ld, ") with the heads of a page contiguous");
-  TORCH_CHECK(state.size(0) <= INT32_MAX, "too many pages");
   fastmax_pages c{};
   c.state = (float*)state.data_ptr();
   c.page_stride = state.size(0) > 1 ? state.stride(0) : pb.heads * rows * ld;
   c.pages = (int32_t)state.size(0);
   if (given(table)) {
-    TORCH_CHECK(table->device() == state.device() && table->scalar_type() == torch::kInt32 && table->is_contiguous() && table->dim() == 1 &&
-                    table->size(0) == pb.batch,
-                "table must be a contiguous int32 tensor with one page per sequence, on the state's device");
+    TORCH_CHECK(table->device() == state.device() && table->scalar_type() == torch::kInt32 && table->is_contiguous(),
+                "table must be a contiguous int32 tensor on the state's device");
     c.table = (const int32_t*)table->data_ptr();
-  } else {
-    TORCH_CHECK(state.size(0) == pb.batch, "without a table the state needs one page per sequence");
   }
   return c;
 }
-// int32 (batch,) on the state's device
-const int32_t* per_sequence(const torch::Tensor& t, const fastmax_problem& pb, const torch::Tensor& like, const char* name) {
-  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.dim() == 1 && t.size(0) == pb.batch, name,
-              " must be a contiguous int32 tensor with one entry per sequence, on the state's device");
+// int32 on the state's device
+const int32_t* numbers_of(const torch::Tensor& t, const torch::Tensor& state, const char* name) {
+  TORCH_CHECK(t.device() == state.device() && t.scalar_type() == torch::kInt32, name, " must be an int32 tensor on the state's device");
   return (const int32_t*)t.data_ptr();
 }
-const int32_t* parents_of(const maybe& parents, const fastmax_problem& pb, const torch::Tensor& like, int64_t& stride) {
-  if (!given(parents)) return nullptr;
-  TORCH_CHECK(parents->device() == like.device() && parents->scalar_type() == torch::kInt32 && parents->dim() == 2 && parents->size(0) == pb.batch &&
-                  parents->size(1) == pb.nq && (pb.nq == 1 || parents->stride(1) == 1),
-              "parents must be an int32 (b, n) tensor with contiguous rows, on the state's device");
-  stride = parents->stride(0);
-  return (const int32_t*)parents->data_ptr();
-}
-// the geometry of (b, h, n, d) tensors of one type on the state's device
-fastmax_problem tree_problem(std::initializer_list<const torch::Tensor*> tensors, const torch::Tensor& state, int64_t p) {
+// the geometry of (b, h, n, d) tensors of one type on the state's device, and what comes with them
+fastmax_problem tree_problem(std::initializer_list<const torch::Tensor*> tensors, const torch::Tensor& state, const maybe& table, int64_t p,
+                             const maybe* parents = nullptr, const torch::Tensor* per_sequence = nullptr) {
   const torch::Tensor& first = **tensors.begin();
-  TORCH_CHECK(first.dim() == 4, "q, k, v must be (b, h, n, d)");
+  TORCH_CHECK_VALUE(state.dim() == 4 && (p == 1 || p == 2), "state must be (pages, heads, rows, d + 4), p 1 or 2");
+  TORCH_CHECK_VALUE(first.dim() == 4 && first.size(1) == state.size(1) && first.size(3) + 4 == state.size(3), "expected (b, ", state.size(1), ", n, ",
+                    state.size(3) - 4, "), got ", first.sizes());
+  const int64_t batch = given(table) ? table->size(0) : state.size(0);
+  TORCH_CHECK_VALUE(first.size(0) == batch, "expected ", batch, " sequences, got ", first.sizes());
+  for (const torch::Tensor* t : tensors) TORCH_CHECK_VALUE(t->sizes() == first.sizes(), "q, k, v and out must have one size, got ", first.sizes(), " and ", t->sizes());
+  TORCH_CHECK(first.numel() > 0 && first.size(2) <= FASTMAX_TREE_NODES, "1 to ", FASTMAX_TREE_NODES, " nodes per sequence, got ", first.sizes());
+  if (parents && given(*parents))
+    TORCH_CHECK_VALUE((*parents)->dim() == 2 && (*parents)->size(0) == batch && (*parents)->size(1) == first.size(2), "parents: expected (b, n) for (b, h, n, d) tensors, got ",
+                      (*parents)->sizes());
+  if (per_sequence) TORCH_CHECK_VALUE(per_sequence->dim() == 1 && per_sequence->size(0) == batch, "one number per sequence expected, got ", per_sequence->sizes());
+  CHECK_CUDA(state);
   for (const torch::Tensor* t : tensors) {
-    CHECK_CUDA((*t));
     TORCH_CHECK(t->device() == state.device(), "the tensors and the state must be on one device");
     TORCH_CHECK(t->scalar_type() == first.scalar_type(), "dtypes differ");
-    TORCH_CHECK(t->sizes() == first.sizes() && (t->size(3) == 1 || t->stride(3) == 1), "q, k, v and out must be (b, h, n, d) of one size, unit stride on the head dim");
+    TORCH_CHECK(t->stride(3) == 1, "the head dim must be contiguous");
   }
-  TORCH_CHECK(first.numel() > 0 && first.size(0) <= INT32_MAX && first.size(1) <= INT32_MAX, "q, k, v must not be empty");
-  TORCH_CHECK(first.size(2) <= FASTMAX_TREE_NODES, "at most ", FASTMAX_TREE_NODES, " nodes per sequence");
   fastmax_problem pb{};
-  pb.batch = first.size(0); pb.heads = first.size(1); pb.nq = pb.nk = first.size(2); pb.d = first.size(3); pb.order = (int)p;
+  pb.batch = batch; pb.heads = first.size(1); pb.nq = pb.nk = first.size(2); pb.d = first.size(3); pb.order = (int)p;
   pb.causal = 1; pb.dtype = dtype_of(first);
-  TORCH_CHECK((pb.d == 16 || pb.d == 32 || pb.d == 64) && (p == 1 || p == 2), "head dim must be 16, 32 or 64, p 1 or 2");
+  TORCH_CHECK(pb.d == 16 || pb.d == 32 || pb.d == 64, "head dim must be 16, 32 or 64");
   return pb;
 }
+// parents with contiguous rows (a copy where they are not)
+torch::Tensor parents_rows(const maybe& parents) {
+  if (!given(parents)) return torch::Tensor();
+  return parents->size(1) == 1 || parents->stride(1) == 1 ? *parents : parents->contiguous();
+}
 
-torch::Tensor tree_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor state, maybe table, maybe parents, maybe lengths,
-                             double inv_temp, double a0, double a1, double a2, int64_t p, maybe out) {
-  fastmax_problem pb = tree_problem({&q, &k, &v}, state, p);
+torch::Tensor tree_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& state, const maybe& table,
+                             const maybe& parents, const maybe& lengths, double inv_temp, double a0, double a1, double a2, int64_t p, const maybe& out) {
+  fastmax_problem pb = given(out) ? tree_problem({&q, &k, &v, &*out}, state, table, p, &parents, given(lengths) ? &*lengths : nullptr)
+                                  : tree_problem({&q, &k, &v}, state, table, p, &parents, given(lengths) ? &*lengths : nullptr);
   pb.a0 = (float)a0; pb.a1 = (float)a1; pb.a2 = (float)a2; pb.inv_temperature = (float)inv_temp;
   const c10::cuda::CUDAGuard guard(q.device());
   fastmax_tree_args a{};
   a.cache = pages_of(state, table, pb);
-  a.parents = parents_of(parents, pb, state, a.parents_stride);
-  if (given(lengths)) a.lengths = per_sequence(*lengths, pb, state, "lengths");
-  torch::Tensor o;
-  if (given(out)) {
-    o = *out;
-    tree_problem({&q, &o}, state, p);
-  } else {
-    // rows that the call does not write are zero
-    o = a.lengths || a.cache.table ? torch::zeros(q.sizes(), q.options()) : torch::empty(q.sizes(), q.options());
-  }
+  const torch::Tensor up = parents_rows(parents), ends = given(lengths) ? lengths->contiguous() : torch::Tensor();
+  if (up.defined()) a.parents = numbers_of(up, state, "parents"), a.parents_stride = up.stride(0);
+  if (ends.defined()) a.lengths = numbers_of(ends, state, "lengths");
+  // without an output of the caller's, rows that the call does not write are zero
+  const torch::Tensor o = given(out)                     ? *out
+                          : a.lengths || a.cache.table ? torch::zeros(q.sizes(), q.options())
+                                                       : torch::empty(q.sizes(), q.options());
   a.q = view_bhnd(q); a.k = view_bhnd(k); a.v = view_bhnd(v); a.o = view_bhnd(o);
   check_status(fastmax_tree_attention(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax tree_attention");
   return o;
 }
 
-void tree_accept(torch::Tensor k, torch::Tensor v, torch::Tensor state, torch::Tensor last, maybe table, maybe parents, int64_t p) {
-  fastmax_problem pb = tree_problem({&k, &v}, state, p);
+void tree_accept(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& state, const torch::Tensor& last, const maybe& table,
+                 const maybe& parents, int64_t p) {
+  fastmax_problem pb = tree_problem({&k, &v}, state, table, p, &parents, &last);
   const c10::cuda::CUDAGuard guard(k.device());
   fastmax_accept_args a{};
   a.cache = pages_of(state, table, pb);
-  a.parents = parents_of(parents, pb, state, a.parents_stride);
-  a.last = per_sequence(last, pb, state, "last");
+  const torch::Tensor up = parents_rows(parents), ends = last.contiguous();
+  if (up.defined()) a.parents = numbers_of(up, state, "parents"), a.parents_stride = up.stride(0);
+  a.last = numbers_of(ends, state, "last");
   a.k = view_bhnd(k); a.v = view_bhnd(v);
   check_status(fastmax_tree_accept(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax tree_accept");
 }
 
-torch::Tensor decode_step_paged(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor state, torch::Tensor table, double inv_temp,
-                                double a0, double a1, double a2, int64_t p, maybe out) {
-  CHECK_CUDA(q);
-  TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q, k, v must be (b, h, d) or (b, h, 1, d)");
+torch::Tensor decode_step_paged(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& state,
+                                const torch::Tensor& table, double inv_temp, double a0, double a1, double a2, int64_t p, const maybe& out) {
   auto rows = [](const torch::Tensor& t) { return t.dim() == 3 ? t.unsqueeze(2) : t; };
-  const torch::Tensor q4 = rows(q), k4 = rows(k), v4 = rows(v);
-  fastmax_problem pb = tree_problem({&q4, &k4, &v4}, state, p);
-  TORCH_CHECK(pb.nq == 1, "one token per (batch, head)");
+  const torch::Tensor q4 = rows(q), k4 = rows(k), v4 = rows(v), given_out = given(out) ? rows(*out) : torch::Tensor();
+  fastmax_problem pb = given_out.defined() ? tree_problem({&q4, &k4, &v4, &given_out}, state, table, p) : tree_problem({&q4, &k4, &v4}, state, table, p);
+  TORCH_CHECK_VALUE(pb.nq == 1, "one token per (batch, head) expected, got ", q.sizes());
   pb.a0 = (float)a0; pb.a1 = (float)a1; pb.a2 = (float)a2; pb.inv_temperature = (float)inv_temp;
   const c10::cuda::CUDAGuard guard(q.device());
-  torch::Tensor o = given(out) ? *out : torch::zeros(q.sizes(), q.options());   // absent sequences' rows are zero
-  const torch::Tensor o4 = rows(o);
-  tree_problem({&q4, &o4}, state, p);
+  const torch::Tensor o = given(out) ? *out : torch::zeros(q.sizes(), q.options());   // absent sequences' rows are zero
   fastmax_paged_decode_args a{};
-  a.q = view_bhnd(q4); a.k = view_bhnd(k4); a.v = view_bhnd(v4); a.o = view_bhnd(o4);
+  a.q = view_bhnd(q4); a.k = view_bhnd(k4); a.v = view_bhnd(v4); a.o = view_bhnd(rows(o));
   a.cache = pages_of(state, table, pb);
   check_status(fastmax_decode_step_paged(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax decode_step");
   return o;
@@ -650,30 +647,33 @@ void check_cache(const torch::Tensor& state, const torch::Tensor& table) {
   TORCH_CHECK(state.size(0) <= FASTMAX_CACHE_PAGES && table.size(0) >= 1 && table.size(0) <= FASTMAX_CACHE_PAGES, "1 to ", FASTMAX_CACHE_PAGES,
               " pages and places");
 }
-torch::Tensor cache_arrange(torch::Tensor state, torch::Tensor table, torch::Tensor sources) {
+// the workspace of a plan and, in front of it, the number it returns
+torch::Tensor plan_workspace(size_t bytes, const torch::Tensor& table) { return torch::empty({(int64_t)(bytes / 4 + 4)}, table.options()); }
+
+torch::Tensor cache_arrange(const torch::Tensor& state, const torch::Tensor& table, const torch::Tensor& given_sources) {
+  TORCH_CHECK_VALUE(given_sources.sizes() == table.sizes(), "sources: expected ", table.sizes(), ", got ", given_sources.sizes());
   check_cache(state, table);
-  TORCH_CHECK(sources.device() == table.device() && sources.scalar_type() == torch::kInt32 && sources.is_contiguous() && sources.sizes() == table.sizes(),
-              "sources must be a contiguous int32 (places,) tensor on the state's device");
   const c10::cuda::CUDAGuard guard(state.device());
+  const torch::Tensor sources = given_sources.contiguous();
+  const int32_t* from = numbers_of(sources, state, "sources");
   const int32_t pages = state.size(0), places = table.size(0);
-  auto unserved = torch::empty({1}, table.options());
   const size_t need = fastmax_cache_workspace(places);
-  auto ws = workspace(need, state);
-  check_status(fastmax_cache_arrange((float*)state.data_ptr(), state.numel() / pages, pages, (int32_t*)table.data_ptr(), places,
-                                     (const int32_t*)sources.data_ptr(), (int32_t*)unserved.data_ptr(), aligned(ws), need,
+  auto ws = plan_workspace(need, table);
+  int32_t* w = (int32_t*)ws.data_ptr();   // from the caching allocator: 16-byte aligned and more
+  check_status(fastmax_cache_arrange((float*)state.data_ptr(), state.numel() / pages, pages, (int32_t*)table.data_ptr(), places, from, w, w + 4, need,
                                      at::cuda::getCurrentCUDAStream().stream()), "fastmax cache_arrange");
-  return unserved;
+  return ws.narrow(0, 0, 1);
 }
-torch::Tensor cache_compact(torch::Tensor state, torch::Tensor table) {
+torch::Tensor cache_compact(const torch::Tensor& state, const torch::Tensor& table) {
   check_cache(state, table);
   const c10::cuda::CUDAGuard guard(state.device());
   const int32_t pages = state.size(0), places = table.size(0);
-  auto live = torch::empty({1}, table.options());
   const size_t need = fastmax_cache_workspace(places);
-  auto ws = workspace(need, state);
-  check_status(fastmax_cache_compact((float*)state.data_ptr(), state.numel() / pages, pages, (int32_t*)table.data_ptr(), places,
-                                     (int32_t*)live.data_ptr(), aligned(ws), need, at::cuda::getCurrentCUDAStream().stream()), "fastmax cache_compact");
-  return live;
+  auto ws = plan_workspace(need, table);
+  int32_t* w = (int32_t*)ws.data_ptr();
+  check_status(fastmax_cache_compact((float*)state.data_ptr(), state.numel() / pages, pages, (int32_t*)table.data_ptr(), places, w, w + 4, need,
+                                     at::cuda::getCurrentCUDAStream().stream()), "fastmax cache_compact");
+  return ws.narrow(0, 0, 1);
 }
 // page dst_index[i] of dst <- page src_index[i] of src (no index: i itself); float32 (pages, ...), the pages contiguous in themselves
 void pages_copy(torch::Tensor src, torch::Tensor dst, maybe src_index, maybe dst_index, int64_t count) {

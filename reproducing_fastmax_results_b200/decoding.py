@@ -80,45 +80,47 @@ class FastmaxDecoder:
         ancestors and itself.  parents: int32 (b, n), the parent of each node (a node before it, or -1: the sequence itself); None: a chain.
         lengths: int32 (b,), nodes of each sequence.  Returns o (b, h, n, d); rows behind a sequence's nodes stay as they are in
         `out`, zero without one."""
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            self._check(t, name)
         return _ext().tree_attention(q, k, v, self.state, None, tree_parents(parents, q), per_sequence(lengths, q, "lengths", 0, q.shape[2]),
                                      self.inv_temperature, self.a0, self.a1, self.a2, self.p, out)
 
     def accept(self, k, v, last, parents=None):
         """Takes drafted tokens into the state: the path from the root to node last[i] for every sequence i, nothing where last[i] is
         -1.  k, v, parents as `verify` had them; last: int32 (b,).  tokens_seen counts the longest path that the drafts can have."""
-        for t, name in ((k, "k"), (v, "v")):
-            self._check(t, name)
         _ext().tree_accept(k, v, self.state, per_sequence(last, k, "last", -1, k.shape[2] - 1), None, tree_parents(parents, k), self.p)
         self.tokens_seen += k.shape[2]
 
 
+def _is_there(x):
+    return x is None or (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.int32)
+
+
 def per_sequence(x, like, name, low, high):
     """One number per sequence as an int32 tensor beside `like`.  What lies on the host is checked to be in low .. high; what lies on the
-    device is not read here (the kernels treat other numbers as their documentation says)."""
-    if x is None:
-        return None
-    x = torch.as_tensor(x)
-    if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
-        raise TypeError(f"{name}: whole numbers expected, got {x.dtype}")
+    device is not read here (the kernels treat other numbers as their documentation says), and int32 there goes on as it is."""
+    if _is_there(x):
+        return x
+    x = _whole(x, name)
     if tuple(x.shape) != (like.shape[0],):
         raise ValueError(f"{name}: expected ({like.shape[0]},), got {tuple(x.shape)}")
     if not x.is_cuda and bool(((x < low) | (x > high)).any()):
         raise ValueError(f"{name}: numbers from {low} to {high} expected")
-    return x.to(device=like.device, dtype=torch.int32).contiguous()
+    return x.to(device=like.device, dtype=torch.int32)
 
 
 def tree_parents(parents, like):
     """The parents of (b, n) nodes as an int32 tensor beside `like` (b, h, n, d); checked as in per_sequence."""
-    if parents is None:
-        return None
-    parents = torch.as_tensor(parents)
-    if parents.dtype.is_floating_point or parents.dtype.is_complex or parents.dtype == torch.bool:
-        raise TypeError(f"parents: whole numbers expected, got {parents.dtype}")
+    if _is_there(parents):
+        return parents
+    parents = _whole(parents, "parents")
     if like.dim() != 4 or tuple(parents.shape) != (like.shape[0], like.shape[2]):
         raise ValueError(f"parents: expected (b, n) for (b, h, n, d) tensors, got {tuple(parents.shape)}")
     if not parents.is_cuda and bool(((parents < -1) | (parents >= torch.arange(parents.shape[1]))).any()):
         raise ValueError("parents: every node needs a parent before it, or -1")
-    parents = parents.to(device=like.device, dtype=torch.int32)
-    return parents if parents.stride(1) == 1 or parents.shape[1] == 1 else parents.contiguous()
+    return parents.to(device=like.device, dtype=torch.int32)
+
+
+def _whole(x, name):
+    x = torch.as_tensor(x)
+    if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
+        raise TypeError(f"{name}: whole numbers expected, got {x.dtype}")
+    return x
