@@ -212,28 +212,31 @@ struct TreeGeo {
   static constexpr int N = 8 * NT;                     // nodes, filled up
   static constexpr int NB = D / 8;
   static constexpr int CG = D / 16;                    // groups of 16 columns of the state: one to a warp
-  static constexpr int KG = NT == 8 || D < 64 ? (D == 16 ? 8 : 4) : 2;   // warps that share a group and divide the rows m of a block among them
+  static constexpr int BLOCKS = NT == 8 && sizeof(T) == 4 ? 1 : 2;   // to an SM
+  static constexpr int KG = D == 16 ? 8 : D == 32 || BLOCKS == 1 ? 4 : 2;   // warps that share a group and divide the rows m of a block among them
   static constexpr int RI = 8 / KG;
   static constexpr int WARPS = CG * KG;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr int BLOCKS = NT == 8 ? 1 : 2;       // to an SM
   static constexpr int LDS = D + 4, C4 = LDS / 4;
   static constexpr int LQ = D + 8;                     // rows of pieces: fragments without bank conflicts
   static constexpr int UNIT = 64 * LDS;                // floats
   static constexpr int QP = Pieces<T>::Q, SP = Pieces<T>::S;
   static constexpr bool HOLD = 2 * NT * QP <= 16;      // a step's fragments of x stay in registers
-  // shared memory in bytes; the place of keys, values and their weights also takes the warps' sums at the end
+  // Shared memory in bytes: slots for units of the state, then what stays for the whole head.  The keys, values, weights and sums of the tree lie
+  // in the last slots until the accumulators start from them, the warps' sums in the first ones at the end.
   static constexpr int PIECES = QP * N * LQ * 2;
   static constexpr int SCALES = D * N * 4;
   static constexpr int ROWS = N * LDS * 4;
-  static constexpr int TREE = PIECES + ROWS + N * N * 4;
+  static constexpr int TREE = PIECES + 2 * ROWS + N * N * 4;
   static constexpr int SUMS = KG * ROWS;
-  static constexpr int SHARED = TREE > SUMS ? TREE : SUMS;
-  static constexpr int FIXED = PIECES + SCALES + ROWS + SHARED + N * 8 + 256;
-  static constexpr int SLOT = (D == 16 ? 64 : D + 1 > 64 ? D + 1 : 64) * LDS * 4;   // a unit, or the linear rows
+  static constexpr int FIXED = PIECES + SCALES + N * 8 + 144;
+  static constexpr int SLOT = (D == 64 ? D + 1 : 64) * LDS * 4;   // a unit, or the linear rows
   static constexpr int ROOM = (BLOCKS == 2 ? 113 : 227) * 1024 - FIXED;
-  static constexpr int SLOTS = ROOM / SLOT > 8 ? 8 : ROOM / SLOT;
-  static constexpr int BYTES = FIXED + SLOTS * SLOT;
+  static constexpr int SLOTS = ROOM / SLOT > 6 ? 6 : ROOM / SLOT;
+  static constexpr int REGION = SLOTS * SLOT > TREE ? (SLOTS * SLOT > SUMS ? SLOTS * SLOT : SUMS) : (TREE > SUMS ? TREE : SUMS);
+  static constexpr int EARLY = (REGION - TREE) / SLOT > SLOTS ? SLOTS : (REGION - TREE) / SLOT;   // slots that are free from the start
+  static constexpr int BYTES = REGION + FIXED;
+  static_assert(BYTES <= 227 * 1024);
   static_assert(SLOTS >= 3);
 };
 
@@ -241,17 +244,16 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(TreeGeo<T, D, NT>::THREADS, TreeGeo<T, D, NT>::BLOCKS)
 attention_kernel(const TreeParams P) {
   using G = TreeGeo<T, D, NT>;
-  constexpr int N = G::N, LDS = G::LDS, C4 = G::C4, LQ = G::LQ, QP = G::QP, SP = G::SP, NB = G::NB, KG = G::KG, RI = G::RI, SLOTS = G::SLOTS, THREADS = G::THREADS;
+  constexpr int N = G::N, LDS = G::LDS, LQ = G::LQ, QP = G::QP, SP = G::SP, NB = G::NB, KG = G::KG, RI = G::RI, SLOTS = G::SLOTS, THREADS = G::THREADS;
   extern __shared__ __align__(128) unsigned char smem[];
-  // [SLOTS][SLOT] units of the state, then
-  __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem + SLOTS * G::SLOT);     // [QP][N][LQ]: pieces of x
-  float* sX = reinterpret_cast<float*>(smem + SLOTS * G::SLOT + G::PIECES);         // [D][N]: x, transposed
-  float* sT = sX + D * N;                                                           // [N][LDS]: the tree's own sums, then the results
+  float* part = reinterpret_cast<float*>(smem);                                     // [KG][N][LDS], at the end in the slots' place
+  float* sT = reinterpret_cast<float*>(smem + G::REGION - G::TREE);                 // [N][LDS], in the last slots' place: the tree's own sums
   float* sV = sT + N * LDS;                                                         // [N][LDS]
   float* sW = sV + N * LDS;                                                         // [N][N]: f of the nodes' pairs
   __nv_bfloat16* sK = reinterpret_cast<__nv_bfloat16*>(sW + N * N);                 // [QP][N][LQ]: pieces of the keys
-  float* part = sV;                                                                 // [KG][N][LDS], in the place of these three
-  unsigned long long* sA = reinterpret_cast<unsigned long long*>(sV + G::SHARED / 4);   // [N]: ancestors
+  __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem + G::REGION);           // [QP][N][LQ]: pieces of x
+  float* sX = reinterpret_cast<float*>(smem + G::REGION + G::PIECES);               // [D][N]: x times the weight of the pairs, transposed
+  unsigned long long* sA = reinterpret_cast<unsigned long long*>(sX + D * N);       // [N]: ancestors
   uint64_t* full = reinterpret_cast<uint64_t*>(sA + N);                                                          // [SLOTS]: a slot's copy has arrived
   int* through = reinterpret_cast<int*>(full + 8);                                  // [SLOTS]: warps that are done with it
   volatile int* issued = reinterpret_cast<volatile int*>(through + 8);              // [SLOTS]: copies that were asked for
@@ -267,6 +269,7 @@ attention_kernel(const TreeParams P) {
     *abort_flag = 0;
     fence_mbar_init();
   }
+  const float c1 = P.a1 * P.inv_t, c2 = P.a2 * P.inv_t * P.inv_t;
   auto meet = [&]() {
     if (CL > 1) cluster.sync();
     else __syncthreads();
@@ -305,7 +308,7 @@ attention_kernel(const TreeParams P) {
     bulk_load(smem + slot * G::SLOT, S + (long long)u * G::UNIT, bytes, &full[slot]);
   };
   if (tid == 0)
-    for (int i = 0; i < SLOTS && u_first + i < u_end; ++i) load(i);
+    for (int i = 0; i < G::EARLY && u_first + i < u_end; ++i) load(i);
   unsigned long long seen[2];   // of nodes lane and lane + 32: warp 0 finds out who sees whom
   int up[2];
   if (warp == 0) {
@@ -329,7 +332,7 @@ attention_kernel(const TreeParams P) {
       rv[t].get(i < n, z);
       *reinterpret_cast<float4*>(sV + i * LDS + c) = make_float4(z[0], z[1], z[2], z[3]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sX[(c + j) * N + i] = x[j];
+      for (int j = 0; j < 4; ++j) sX[(c + j) * N + i] = c2 * x[j];
       uint32_t p0[QP], p1[QP];
       split2(x[0], x[1], p0);
       split2(x[2], x[3], p1);
@@ -430,13 +433,30 @@ attention_kernel(const TreeParams P) {
       }
     }
     *reinterpret_cast<float4*>(sT + i * LDS + c) = sum;
-    if (c == 0) *reinterpret_cast<float4*>(sT + i * LDS + D) = make_float4(total, 0.f, 0.f, 0.f);
+    if (c == 0) sT[i * LDS + D] = total;
   }
 
   // ---- the state --------------------------------------------------------------------------------------------------------------
   const int kg = warp / G::CG, column = 16 * (warp % G::CG) + 2 * g;   // this warp's rows m, this thread's two columns
-  const float c1 = P.a1 * P.inv_t, c2 = P.a2 * P.inv_t * P.inv_t;
   float acc[NT][4] = {}, den[NT][2] = {};
+  __syncthreads();
+  if (kg == 0) {   // this block's nodes start from the tree's sums
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 8 * nt + t2 + e - i0;
+        if (i < 0 || i >= mine) continue;
+        const float2 x = *reinterpret_cast<const float2*>(sT + i * LDS + column);
+        acc[nt][e] = x.x, acc[nt][2 + e] = x.y;
+        if (warp == 0 && g == 0) den[nt][e] = sT[i * LDS + D];
+      }
+  }
+  __syncthreads();   // nobody reads what the tree needed any more
+  if (tid == 0) {
+    fence_proxy_async_smem();
+    for (int i = G::EARLY; i < SLOTS && u_first + i < u_end; ++i) load(i);
+  }
   // pieces of two rows of two columns (of the product: rows g and g + 8)
   auto s_pieces = [&](uint32_t (&a)[SP][4], int half, const float* at) {
     const float2 x = *reinterpret_cast<const float2*>(at), y = *reinterpret_cast<const float2*>(at + LDS);
@@ -535,12 +555,6 @@ attention_kernel(const TreeParams P) {
     done += pair ? 2 : 1, ub += pair ? 2 : 1, ++step;
     if (ub >= NB) ++ua, ub = ua;
   }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {   // the weight of all pairs
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[nt][j] *= c2;
-    den[nt][0] *= c2, den[nt][1] *= c2;
-  }
   if (u_end > npairs) {
     // the linear rows, x_m S[m], 16 of them a warp, and the constant's row
     const float* U = unit(done);
@@ -579,7 +593,7 @@ attention_kernel(const TreeParams P) {
       }
     }
   }
-  __syncthreads();   // nobody reads values and weights any more
+  __syncthreads();   // nobody reads the state any more
   if (tid == 0 && *abort_flag != 0)   // leave only after the copies in flight
     for (int i = 0; i < SLOTS; ++i)
       if (issued[i] > 0) mbar_wait_bounded(&full[i], (uint32_t)(issued[i] - 1) & 1u, WAIT_CYCLES);
@@ -599,29 +613,24 @@ attention_kernel(const TreeParams P) {
       }
     }
   meet();
-  for (int idx = tid; idx < mine * C4; idx += THREADS) {
-    const int i = idx / C4, c = 4 * (idx - i * C4);
-    float4 x = *reinterpret_cast<const float4*>(sT + i * LDS + c);
-    for (int r = 0; r < CL; ++r) {
-      const float* sums = (CL > 1 ? cluster.map_shared_rank(part, r) : part) + (i0 + i) * LDS + c;
-#pragma unroll
-      for (int w = 0; w < KG; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(sums + w * N * LDS);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-      }
-    }
-    *reinterpret_cast<float4*>(sT + i * LDS + c) = x;
-  }
-  meet();   // (also: nobody's sums are read any more)
   T* o = const_cast<T*>(head_base<T>(P.o, head, P.heads));
   for (int idx = tid; idx < mine * (D / 4); idx += THREADS) {
-    const int i = idx / (D / 4), c = 4 * (idx - i * (D / 4));
-    const float4 last = *reinterpret_cast<const float4*>(sT + i * LDS + D);
+    const int i = i0 + idx / (D / 4), c = 4 * (idx % (D / 4));
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), last = x;
+    for (int r = 0; r < CL; ++r) {
+      const float* sums = (CL > 1 ? cluster.map_shared_rank(part, r) : part) + i * LDS;
+#pragma unroll
+      for (int w = 0; w < KG; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(sums + w * N * LDS + c), z = *reinterpret_cast<const float4*>(sums + w * N * LDS + D);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        last.x += z.x, last.y += z.y, last.z += z.z, last.w += z.w;
+      }
+    }
     const float total = (last.x + last.y) + (last.z + last.w);
-    const float4 x = *reinterpret_cast<const float4*>(sT + i * LDS + c);
-    store4v(o + (i0 + i) * P.o.sn + c, P.aligned, x.x / total, x.y / total, x.z / total, x.w / total);
-    if (c == 0 && P.g.ptr != nullptr) const_cast<float*>(head_base<float>(P.g, head, P.heads))[(i0 + i) * P.g.sn] = total;
+    store4v(o + i * P.o.sn + c, P.aligned, x.x / total, x.y / total, x.z / total, x.w / total);
+    if (c == 0 && P.g.ptr != nullptr) const_cast<float*>(head_base<float>(P.g, head, P.heads))[i * P.g.sn] = total;
   }
+  if (CL > 1) cluster.sync();   // nobody's sums are read any more
 }
 
 // ---- taking a path ---------------------------------------------------------------------------------------------------------
@@ -640,7 +649,7 @@ __global__ void __launch_bounds__(AcceptGeo<D>::THREADS)
 accept_kernel(const TreeParams P, int units_each) {
   using G = AcceptGeo<D>;
   constexpr int C4 = G::C4, LV = G::LV, NB = D / 8, THREADS = G::THREADS;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   float* sK = reinterpret_cast<float*>(smem);              // [nodes][D]: keys of the path, from the root down
   float* sV = sK + P.nodes * D;                            // [nodes][LV]: [v | 1 0 0 0]
   int* path = reinterpret_cast<int*>(sV + P.nodes * LV);   // [nodes]
