@@ -209,14 +209,17 @@ typedef struct {
                         /* sequence is absent: nothing of it is read or written.  NULL: sequence b has page b (pages >= batch)  */
 } fastmax_pages;
 
-/* fastmax_decode_step with a page per sequence.  The outputs of absent sequences stay as they were. */
+/* fastmax_decode_step with a page per sequence.  The outputs of absent sequences stay as they were.  workspace:
+ * fastmax_decode_step_workspace(pb) bytes, 16-byte aligned, not to be shared by calls that may overlap; 0 for few heads.  One launch, or two. */
 typedef struct {
   fastmax_tensor q, k, v;
   fastmax_tensor o;
   fastmax_tensor g;
   fastmax_pages cache;
 } fastmax_paged_decode_args;
-int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged_decode_args* args, void* cuda_stream);
+size_t fastmax_decode_step_workspace(const fastmax_problem* pb);
+int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged_decode_args* args, void* workspace, size_t workspace_bytes,
+                                  void* cuda_stream);
 
 /* Attention of a tree of drafted tokens over the cached sequence, which stays as it is:
  *     o_i = ( sum_r w_r Phi(q_i)_r S[r] + sum_{j in A(i)} f(q_i . k_j * inv_temperature) [v_j | 1] ), divided by its last element,

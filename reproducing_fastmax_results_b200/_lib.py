@@ -22,7 +22,7 @@ EXPORTED_SYMBOLS = [
     "fastmax_forward_workspace", "fastmax_forward", "fastmax_key_moments_bytes", "fastmax_forward_engine",
     "fastmax_static_scratch_bytes", "fastmax_forward_static_scratch",
     "fastmax_backward_workspace", "fastmax_backward", "fastmax_backward_key_moments_bytes", "fastmax_grad_moments_bytes",
-    "fastmax_decode_step", "fastmax_decode_step_paged", "fastmax_tree_attention", "fastmax_tree_accept",
+    "fastmax_decode_step", "fastmax_decode_step_workspace", "fastmax_decode_step_paged", "fastmax_tree_attention", "fastmax_tree_accept",
     "fastmax_pages_copy", "fastmax_cache_workspace", "fastmax_cache_arrange", "fastmax_cache_compact",
     "fastmax_normalize_forward", "fastmax_normalize_backward",
     "fastmax_key_prologue", "fastmax_output_noise",
@@ -149,7 +149,9 @@ def load():
     lib.fastmax_decode_step.restype = C.c_int32
     lib.fastmax_decode_step.argtypes = [C.POINTER(Problem), C.POINTER(DecodeArgs), C.c_void_p]
     lib.fastmax_decode_step_paged.restype = C.c_int32
-    lib.fastmax_decode_step_paged.argtypes = [C.POINTER(Problem), C.POINTER(PagedDecodeArgs), C.c_void_p]
+    lib.fastmax_decode_step_paged.argtypes = [C.POINTER(Problem), C.POINTER(PagedDecodeArgs), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.fastmax_decode_step_workspace.restype = C.c_size_t
+    lib.fastmax_decode_step_workspace.argtypes = [C.POINTER(Problem)]
     lib.fastmax_tree_attention.restype = C.c_int32
     lib.fastmax_tree_attention.argtypes = [C.POINTER(Problem), C.POINTER(TreeArgs), C.c_void_p]
     lib.fastmax_tree_accept.restype = C.c_int32
@@ -407,7 +409,9 @@ def decode_step_paged(q, k, v, state, table, inv_temp, a0=1.0, a1=1.0, a2=0.5, o
     args.q, args.k, args.v, args.o = (Tensor(t.data_ptr(), t.stride(0), t.stride(1), 0) for t in (q, k, v, o))
     args.g = Tensor(g.data_ptr(), g.stride(0), g.stride(1), 0)
     args.cache = _pages(state, table)
-    check(lib.fastmax_decode_step_paged(C.byref(pb), C.byref(args), _stream()), "fastmax_decode_step_paged")
+    need = lib.fastmax_decode_step_workspace(C.byref(pb))
+    ws, wptr = _workspace(need, q.device)
+    check(lib.fastmax_decode_step_paged(C.byref(pb), C.byref(args), wptr, need, _stream()), "fastmax_decode_step_paged")
     return o, g
 
 

@@ -207,6 +207,150 @@ decode_step_kernel(const DecodeParams P) {
   }
 }
 
+// ---- many heads, on pages ----------------------------------------------------------------------------------------------------
+// The same step as short blocks without clusters: a block has four units of one head (a unit: the 64 products of a pair of blocks, or the linear
+// rows), a thread one float4 column of four rows (m .. m + 3, n) of a unit and the next unit's four in flight; the parts of the outputs go through
+// the workspace and a second, small launch adds them in the units' order and divides.
+template <int D>
+struct RowsGeo {
+  static constexpr int C4 = (D + 4) / 4;
+  static constexpr int THREADS = 16 * C4;
+  static constexpr int EACH = 4;   // units
+};
+__host__ __device__ inline int row_groups(int d, int order) { return ((order == 2 ? (d / 8) * (d / 8 + 1) / 2 : 0) + 1 + 3) / 4; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(RowsGeo<D>::THREADS)
+step_rows_kernel(const DecodeParams P, float4* parts) {
+  using G = RowsGeo<D>;
+  constexpr int C4 = G::C4, NB = D / 8;
+  __shared__ __align__(16) float sq[D], sk[D];
+  __shared__ float4 red[16][C4];
+  const int tid = threadIdx.x, head = blockIdx.y, bi = head / P.heads, hi = head - bi * P.heads;
+  const int npairs = (P.rows - D - 1) / 64;
+  const int u0 = blockIdx.x * G::EACH, u1 = min(u0 + G::EACH, npairs + 1);
+  grid_wait();
+  grid_trigger();
+  long long first = (long long)bi * P.page_stride + (long long)hi * (P.rows * (D + 4));
+  if (P.table != nullptr) {
+    const int page = P.table[bi];
+    if (page < 0 || page >= P.pages) return;
+    first += (long long)(page - bi) * P.page_stride;
+  }
+  const int c4 = tid % C4, rg = tid / C4;
+  const int n8 = rg & 7, m8 = 4 * (rg >> 3);
+  float4* base = reinterpret_cast<float4*>(P.state + first) + c4;
+  auto row_of = [&](int u, int j) { return u < npairs ? 64 * u + 8 * (m8 + j) + n8 : 64 * npairs + rg + 16 * j; };
+  auto there = [&](int u, int j) { return u < npairs || rg + 16 * j < D; };
+  float4 next[4], ones = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto fetch = [&](int u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (there(u, j)) next[j] = __ldcs(base + (long long)row_of(u, j) * C4);
+    if (u == npairs && rg == 0) ones = __ldcs(base + (long long)(64 * npairs + D) * C4);   // the constant's row
+  };
+  fetch(u0);
+  if (tid < D) {
+    sq[tid] = to_f<T>(reinterpret_cast<const T*>(P.q.ptr)[(long long)bi * P.q.sb + (long long)hi * P.q.sh + tid]);
+    sk[tid] = to_f<T>(reinterpret_cast<const T*>(P.k.ptr)[(long long)bi * P.k.sb + (long long)hi * P.k.sh + tid]);
+  }
+  float4 v4 = make_float4(1.f, 0.f, 0.f, 0.f);
+  if (c4 < D / 4) {
+    const T* vp = reinterpret_cast<const T*>(P.v.ptr) + (long long)bi * P.v.sb + (long long)hi * P.v.sh + 4 * c4;
+    v4 = make_float4(to_f<T>(vp[0]), to_f<T>(vp[1]), to_f<T>(vp[2]), to_f<T>(vp[3]));
+  }
+  __syncthreads();
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto update = [&](float4& s, float pk, float pq) {
+    s.x = fmaf(pk, v4.x, s.x), s.y = fmaf(pk, v4.y, s.y), s.z = fmaf(pk, v4.z, s.z), s.w = fmaf(pk, v4.w, s.w);
+    acc.x = fmaf(pq, s.x, acc.x), acc.y = fmaf(pq, s.y, acc.y), acc.z = fmaf(pq, s.z, acc.z), acc.w = fmaf(pq, s.w, acc.w);
+  };
+  int ua = 0, ub = 0;
+  if (u0 < npairs) pair_decode(u0, NB, ua, ub);
+  for (int u = u0; u < u1; ++u) {
+    float4 s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = next[j];
+    if (u + 1 < u1) fetch(u + 1);
+    if (u < npairs) {
+      const float4 km = *reinterpret_cast<const float4*>(sk + 8 * ua + m8), qm = *reinterpret_cast<const float4*>(sq + 8 * ua + m8);
+      const float kn = sk[8 * ub + n8], qn = sq[8 * ub + n8], weight = ua == ub ? P.c2 : 2.f * P.c2;
+      update(s[0], km.x * kn, qm.x * qn * weight);
+      update(s[1], km.y * kn, qm.y * qn * weight);
+      update(s[2], km.z * kn, qm.z * qn * weight);
+      update(s[3], km.w * kn, qm.w * qn * weight);
+      if (++ub == NB) ub = ++ua;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (there(u, j)) update(s[j], sk[rg + 16 * j], sq[rg + 16 * j] * P.c1);
+      if (rg == 0) {
+        update(ones, 1.f, P.c0);
+        __stcs(base + (long long)(64 * npairs + D) * C4, ones);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (there(u, j)) __stcs(base + (long long)row_of(u, j) * C4, s[j]);
+  }
+  red[rg][c4] = acc;
+  __syncthreads();
+  if (tid < C4) {
+    float4 t = red[0][tid];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) {
+      const float4 x = red[j][tid];
+      t.x += x.x, t.y += x.y, t.z += x.z, t.w += x.w;
+    }
+    parts[((long long)head * gridDim.x + blockIdx.x) * C4 + tid] = t;
+  }
+}
+
+template <typename T, int D>
+__global__ void step_divide_kernel(const DecodeParams P, const float* parts, int groups, int total) {
+  constexpr int LD = D + 4;
+  grid_wait();
+  grid_trigger();
+  const int head = blockIdx.x * blockDim.y + threadIdx.y, c = threadIdx.x;   // a column of the state
+  __shared__ float sums[256 / D];
+  float x = 0.f, g = 0.f;
+  int bi = 0, hi = 0;
+  bool live = head < total;
+  if (live) {
+    bi = head / P.heads, hi = head - bi * P.heads;
+    live = P.table == nullptr || (P.table[bi] >= 0 && P.table[bi] < P.pages);
+  }
+  if (live) {
+    const float* at = parts + (long long)head * groups * LD;
+    for (int i = 0; i < groups; ++i) x += at[i * LD + c];
+    if (c == 0) {
+      for (int i = 0; i < groups; ++i) g += at[i * LD + D];
+      sums[threadIdx.y] = g;
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  T* op = reinterpret_cast<T*>(const_cast<void*>(P.o.ptr)) + (long long)bi * P.o.sb + (long long)hi * P.o.sh;
+  op[c] = from_f<T>(x / sums[threadIdx.y]);
+  if (c == 0 && P.g.ptr != nullptr)
+    *(reinterpret_cast<float*>(const_cast<void*>(P.g.ptr)) + (long long)bi * P.g.sb + (long long)hi * P.g.sh) = g;
+}
+
+template <typename T, int D>
+static cudaError_t launch_rows(int order, const DecodeParams& P, int bh, float* parts, cudaStream_t st) {
+  const int groups = row_groups(D, order);
+  cudaError_t e = launch_after(step_rows_kernel<T, D>, dim3((unsigned)groups, (unsigned)bh), RowsGeo<D>::THREADS, 0, st, P, reinterpret_cast<float4*>(parts));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((bh + 256 / D - 1) / (256 / D)));
+  cfg.blockDim = dim3(D, 256 / D);
+  cfg.stream = st;
+  cudaLaunchAttribute attr = launch_attribute_after();
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return launched(cudaLaunchKernelEx(&cfg, step_divide_kernel<T, D>, P, (const float*)parts, groups, bh));
+}
+
 template <int D, int RG>
 static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int bh, int cl, cudaStream_t st) {
   cfg.gridDim = dim3(cl, bh);
@@ -260,7 +404,14 @@ static cudaError_t launch(int order, const DecodeParams& P, int bh, cudaStream_t
 }
 
 template <typename T>
-static cudaError_t launch_d(int d, int order, const DecodeParams& P, int bh, cudaStream_t st) {
+static cudaError_t launch_d(int d, int order, const DecodeParams& P, int bh, float* parts, cudaStream_t st) {
+  if (parts != nullptr) {
+    switch (d) {
+      case 16: return launch_rows<T, 16>(order, P, bh, parts, st);
+      case 32: return launch_rows<T, 32>(order, P, bh, parts, st);
+      default: return launch_rows<T, 64>(order, P, bh, parts, st);
+    }
+  }
   switch (d) {
     case 16: return launch<T, 16>(order, P, bh, st);
     case 32: return launch<T, 32>(order, P, bh, st);
@@ -271,7 +422,8 @@ static cudaError_t launch_d(int d, int order, const DecodeParams& P, int bh, cud
 }  // namespace dec
 }  // namespace fm
 
-extern "C" int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged_decode_args* a, void* cuda_stream) {
+// parts: NULL, or the workspace of the form for many heads
+static int32_t decode_step(const fastmax_problem* pb, const fastmax_paged_decode_args* a, float* parts, void* cuda_stream) {
   using namespace fm;
   if (!pb || !a) return FASTMAX_ERR_INVALID_ARGUMENT;
   if (pb->batch <= 0 || pb->heads <= 0) return FASTMAX_ERR_INVALID_ARGUMENT;
@@ -302,10 +454,27 @@ extern "C" int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fa
   cudaError_t e;
   {
     LaunchScope ls(KK_DECODE, st);
-    e = pb->dtype == FASTMAX_BF16 ? dec::launch_d<__nv_bfloat16>(pb->d, pb->order, P, bh, st)
-                                  : dec::launch_d<float>(pb->d, pb->order, P, bh, st);
+    e = pb->dtype == FASTMAX_BF16 ? dec::launch_d<__nv_bfloat16>(pb->d, pb->order, P, bh, parts, st)
+                                  : dec::launch_d<float>(pb->d, pb->order, P, bh, parts, st);
   }
   return e == cudaSuccess ? FASTMAX_OK : report_cuda_error(e);
+}
+
+extern "C" size_t fastmax_decode_step_workspace(const fastmax_problem* pb) {
+  using namespace fm;
+  if (!pb || pb->batch <= 0 || pb->heads <= 0 || (pb->d != 16 && pb->d != 32 && pb->d != 64) || (pb->order != 1 && pb->order != 2)) return 0;
+  const long long bh = (long long)pb->batch * pb->heads;
+  // us by clusters / by short blocks: d = 64, 64 heads 19.7 / 19.7, 128 36.1 / 31.8, 512 115.7 / 106.1; d = 32, 64 heads 7.0 / 8.5, 128 12.4 / 10.2,
+  // 512 27.9 / 22.2; d = 16, 512 heads 7.3 / 8.3; order 1, d = 64, 512 heads 9.6 / 8.6.
+  if (pb->d < 32 || bh < (pb->order == 2 ? 128 : 512)) return 0;
+  return (size_t)(bh * dec::row_groups(pb->d, pb->order) * state_ld(pb->d) * 4);
+}
+
+extern "C" int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged_decode_args* a, void* workspace, size_t workspace_bytes,
+                                             void* cuda_stream) {
+  const size_t need = fastmax_decode_step_workspace(pb);
+  if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < need)) return FASTMAX_ERR_WORKSPACE;
+  return decode_step(pb, a, need > 0 ? reinterpret_cast<float*>(workspace) : nullptr, cuda_stream);
 }
 
 extern "C" int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_decode_args* a, void* cuda_stream) {
@@ -315,5 +484,5 @@ extern "C" int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_
   paged.cache.state = a->state;
   paged.cache.page_stride = (int64_t)pb->heads * fm::state_rows(pb->d, pb->order) * fm::state_ld(pb->d);
   paged.cache.pages = pb->batch;
-  return fastmax_decode_step_paged(pb, &paged, cuda_stream);
+  return decode_step(pb, &paged, nullptr, cuda_stream);
 }

@@ -634,7 +634,9 @@ torch::Tensor decode_step_paged(const torch::Tensor& q, const torch::Tensor& k, 
   fastmax_paged_decode_args a{};
   a.q = view_bhnd(q4); a.k = view_bhnd(k4); a.v = view_bhnd(v4); a.o = view_bhnd(rows(o));
   a.cache = pages_of(state, table, pb);
-  check_status(fastmax_decode_step_paged(&pb, &a, at::cuda::getCurrentCUDAStream().stream()), "fastmax decode_step");
+  const size_t need = fastmax_decode_step_workspace(&pb);
+  const torch::Tensor ws = need > 0 ? torch::empty({(int64_t)need}, q.options().dtype(torch::kUInt8)) : torch::Tensor();   // 16-byte aligned and more
+  check_status(fastmax_decode_step_paged(&pb, &a, need > 0 ? ws.data_ptr() : nullptr, need, at::cuda::getCurrentCUDAStream().stream()), "fastmax decode_step");
   return o;
 }
 

@@ -248,6 +248,42 @@ def test_steps_on_pages_are_the_steps_of_a_dense_state(heads, dtype):
         assert torch.equal(cache[:, 0], before[:, 0]) and torch.equal(cache[1:4], before[1:4])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,heads,d,order", [(9, 16, 64, 2), (16, 8, 64, 2), (17, 8, 32, 2), (40, 13, 64, 1), (33, 16, 32, 1), (60, 16, 16, 2)])
+def test_steps_of_many_heads_on_pages(batch, heads, d, order, dtype):
+    from reproducing_fastmax_results_b200 import _lib as L
+
+    gen = torch.Generator(device="cuda").manual_seed(batch)
+    cache = states(batch + 1, heads, d, order, gen, layers=2)
+    before = cache.clone()
+    table = np.random.default_rng(batch).permutation(batch + 1)[:batch]
+    table[[1, batch - 1]] = [-1, batch + 1]
+    qkv = torch.randn(batch, 3, heads, d, device="cuda", generator=gen).to(dtype)
+    qkv[1] = float("nan")
+    q, k, v = qkv.unbind(1)
+    out = torch.full((batch, heads, d), 3.0, device="cuda").to(dtype)
+    o, g = L.decode_step_paged(q, k, v, cache[:, 0], i32(table), 0.1, *A, order, out=out)
+    for i in (0, 1, 2, batch // 2, batch - 2, batch - 1):
+        page = int(table[i])
+        if not 0 <= page <= batch:
+            assert (o[i] == 3.0).all() and (g[i] == 0).all()
+            continue
+        for j in (0, heads - 1):
+            old, new = host(before[page, 0, j]), host(cache[page, 0, j])
+            kk, vv, qq = (host(t[i, j])[None] for t in (k, v, q))
+            ref, size = so.grown(old, kk, vv, order)
+            assert (np.abs(new[:, : d + 1] - ref) <= so.grown_tolerance(size, 1)).all() and (new[:, d + 1:] == old[:, d + 1:]).all()
+            oref, gref, osize, gsize = so.tree(qq, kk, vv, old, [-1], order, A, 0.1)
+            rounding = 2.0 ** (-8 if dtype == torch.bfloat16 else -24)
+            assert (np.abs(host(o[i, j])[None] - oref) <= rounding * np.abs(oref) + so.SUMS_F32 * osize).all()
+            assert abs(float(g[i, j]) - gref[0]) <= so.SUMS_F32 * gsize[0]
+    rest = sorted(set(range(batch + 1)) - set(table.tolist()))
+    assert torch.equal(cache[:, 1], before[:, 1]) and torch.equal(cache[rest], before[rest])
+    again = before.clone()   # the same bits on every run
+    o2, _ = L.decode_step_paged(q, k, v, again[:, 0], i32(table), 0.1, *A, order, out=torch.full_like(out, 3.0))
+    assert torch.equal(o2, o) and torch.equal(again, cache)
+
+
 # ---- pages -----------------------------------------------------------------------------------------------------------------
 def arrange_and_compare(table, sources, pages, floats, seed):
     from reproducing_fastmax_results_b200.attention import _ext

@@ -47,7 +47,7 @@ def calls(pb, c, missing=None):
     single = L.Problem.from_buffer_copy(pb)
     if pb.nq == pb.nk == 5:
         single.nq = single.nk = 1
-    yield "step", lib.fastmax_decode_step_paged(C.byref(single), C.byref(one), None)
+    yield "step", lib.fastmax_decode_step_paged(C.byref(single), C.byref(one), PTR, 1 << 40, None)
     yield "verify", lib.fastmax_tree_attention(C.byref(pb), C.byref(tree), None)
     yield "accept", lib.fastmax_tree_accept(C.byref(pb), C.byref(accept), None)
 
@@ -79,6 +79,19 @@ def test_missing_tensors_are_refused(missing, by):
     # the others would be launched: a misaligned state stops them before that
     for name, got in calls(problem(), cache(state=PTR + 8), missing):
         assert got == (1 if name in by else 6), name
+
+
+def test_a_step_without_its_workspace_is_refused():
+    lib = L.load()
+    assert lib.fastmax_decode_step_workspace(C.byref(problem())) == lib.fastmax_decode_step_workspace(None) == 0
+    many = problem(batch=60, nq=1, nk=1)   # 180 heads
+    need = lib.fastmax_decode_step_workspace(C.byref(many))
+    assert need >= 180 * 3 * 36 * 4
+    args = L.PagedDecodeArgs()
+    args.q = args.k = args.v = args.o = L.Tensor(PTR, 96, 32, 0)
+    args.cache = cache(pages=60, state=PTR + 8)
+    for ws, nbytes, status in ((None, need, 3), (PTR + 8, need, 3), (PTR, need - 1, 3), (PTR, need, 6)):
+        assert lib.fastmax_decode_step_paged(C.byref(many), C.byref(args), ws, nbytes, None) == status
 
 
 def test_page_moves_are_refused():
