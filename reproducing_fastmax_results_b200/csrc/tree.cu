@@ -120,10 +120,32 @@ __device__ __forceinline__ void store4v(__nv_bfloat16* p, bool aligned, float a,
   }
 }
 
-__device__ __forceinline__ int parent_of(const TreeParams& P, int b, int i) {
-  if (P.parents == nullptr) return i - 1;
-  const int p = P.parents[b * P.parents_stride + i];
-  return p >= 0 && p < i ? p : -1;
+// Who sees whom, by one warp: of nodes lane and lane + 32 the node itself and its ancestors as bits.  `up`: their parents.  Pointers reach
+// twice as far in every round.
+__device__ __forceinline__ void load_parents(const TreeParams& P, int b, int lane, int (&up)[2]) {   // as they stand there
+#pragma unroll
+  for (int k = 0; k < 2; ++k) up[k] = P.parents != nullptr && lane + 32 * k < P.nodes ? P.parents[b * P.parents_stride + lane + 32 * k] : -1;
+}
+__device__ __forceinline__ void ancestors(const TreeParams& P, int n, int lane, int (&up)[2], unsigned long long (&seen)[2]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) seen[k] = P.parents == nullptr ? (2ull << (lane + 32 * k)) - 1ull : 1ull << (lane + 32 * k);
+  if (P.parents == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (up[k] >= lane + 32 * k || up[k] < 0) up[k] = -1;   // no node before it
+  for (int far = 1; far < n; far *= 2) {
+    unsigned long long more[2];
+    int next[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned long long m0 = __shfl_sync(0xffffffffu, seen[0], up[k] & 31), m1 = __shfl_sync(0xffffffffu, seen[1], up[k] & 31);
+      const int n0 = __shfl_sync(0xffffffffu, up[0], up[k] & 31), n1 = __shfl_sync(0xffffffffu, up[1], up[k] & 31);
+      more[k] = up[k] < 0 ? 0ull : up[k] < 32 ? m0 : m1;
+      next[k] = up[k] < 0 ? -1 : up[k] < 32 ? n0 : n1;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) seen[k] |= more[k], up[k] = next[k];
+  }
 }
 // first float of the sequence's head, or NULL for an absent sequence
 __device__ __forceinline__ float* head_state(const TreeParams& P, int b, int h, int d) {
@@ -309,16 +331,8 @@ attention_kernel(const TreeParams P) {
   };
   if (tid == 0)
     for (int i = 0; i < G::EARLY && u_first + i < u_end; ++i) load(i);
-  unsigned long long seen[2];   // of nodes lane and lane + 32: warp 0 finds out who sees whom
-  int up[2];
-  if (warp == 0) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = lane + 32 * k;
-      seen[k] = P.parents == nullptr ? (2ull << i) - 1ull : 1ull << i;
-      up[k] = P.parents == nullptr || i >= n ? -1 : parent_of(P, b, i);
-    }
-  }
+  int up[2];   // warp 0 finds out who sees whom
+  if (warp == 0) load_parents(P, b, lane, up);
 
   // ---- x, keys, values ----------------------------------------------------------------------------------------------------------
   {
@@ -345,21 +359,8 @@ attention_kernel(const TreeParams P) {
     }
   }
   if (warp == 0) {
-    if (P.parents != nullptr) {
-      for (int far = 1; far < n; far *= 2) {   // pointers twice as far up in every round
-        unsigned long long more[2];
-        int next[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const unsigned long long m0 = __shfl_sync(0xffffffffu, seen[0], up[k] & 31), m1 = __shfl_sync(0xffffffffu, seen[1], up[k] & 31);
-          const int n0 = __shfl_sync(0xffffffffu, up[0], up[k] & 31), n1 = __shfl_sync(0xffffffffu, up[1], up[k] & 31);
-          more[k] = up[k] < 0 ? 0ull : up[k] < 32 ? m0 : m1;
-          next[k] = up[k] < 0 ? -1 : up[k] < 32 ? n0 : n1;
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) seen[k] |= more[k], up[k] = next[k];
-      }
-    }
+    unsigned long long seen[2];
+    ancestors(P, n, lane, up, seen);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (lane + 32 * k < N) sA[lane + 32 * k] = seen[k];
@@ -640,27 +641,27 @@ template <int D>
 struct AcceptGeo {
   static constexpr int C4 = (D + 4) / 4;
   static constexpr int THREADS = 16 * C4;              // 64 rows of a unit, four to a thread
+  static constexpr int BLOCKS = D == 64 ? 3 : D == 32 ? 5 : 9;   // to an SM: two of 64 dims take 117 us for 512 heads where three take 101
   static constexpr int LV = D + 4;
-  static int bytes(int nodes) { return nodes * (D + LV) * 4 + nodes * 8; }
+  static int bytes(int nodes) { return nodes * (D + LV) * 4; }
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(AcceptGeo<D>::THREADS)
+__global__ void __launch_bounds__(AcceptGeo<D>::THREADS, AcceptGeo<D>::BLOCKS)
 accept_kernel(const TreeParams P, int units_each) {
   using G = AcceptGeo<D>;
-  constexpr int C4 = G::C4, LV = G::LV, NB = D / 8, THREADS = G::THREADS;
+  constexpr int C4 = G::C4, LV = G::LV, NB = D / 8;
   extern __shared__ __align__(128) unsigned char smem[];
   float* sK = reinterpret_cast<float*>(smem);              // [nodes][D]: keys of the path, from the root down
   float* sV = sK + P.nodes * D;                            // [nodes][LV]: [v | 1 0 0 0]
-  int* path = reinterpret_cast<int*>(sV + P.nodes * LV);   // [nodes]
-  int* up = path + P.nodes;                                // [nodes]
-  __shared__ int length;
   const int tid = threadIdx.x, head = blockIdx.y, b = head / P.heads;
   const int npairs = P.order == 2 ? Geo<D>::NPAIRS : 0;
   const int u0 = blockIdx.x * units_each, u1 = min(u0 + units_each, npairs + 1);
   grid_wait();
   grid_trigger();
-  const int last = P.ends[b];
+  int up[2];
+  if (tid < 32) load_parents(P, b, tid, up);
+  const int last = P.ends[b];   // (in flight beside the parents and the table's entry)
   float* S = head_state(P, b, head - b * P.heads, D);
   if (S == nullptr || last < 0 || last >= P.nodes) return;
 
@@ -669,44 +670,44 @@ accept_kernel(const TreeParams P, int units_each) {
   auto row_of = [&](int u, int j) { return u < npairs ? 64 * u + 8 * (m8 + j) + n8 : 64 * npairs + rg + 16 * j; };
   auto there = [&](int u, int j) { return u < npairs || rg + 16 * j < D; };
   float4* base = reinterpret_cast<float4*>(S) + c4;
-  float4 next[4], ones = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 next[4];
   auto fetch = [&](int u) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (there(u, j)) next[j] = __ldcs(base + (long long)row_of(u, j) * C4);
-    if (u == npairs && rg == 0) ones = __ldcs(base + (long long)(64 * npairs + D) * C4);   // the constant's row
   };
   fetch(u0);
-  if (P.parents != nullptr)
-    for (int i = tid; i <= last; i += THREADS) up[i] = parent_of(P, b, i);
-  __syncthreads();
-  if (tid == 0) {
-    int n = 0;
-    if (P.parents == nullptr) {
-      n = last + 1;
-    } else {
-      for (int i = last; i >= 0; i = up[i]) path[n++] = i;
+  // the path from the root down: parents come before their children, so it is the ancestors' bits in their order
+  __shared__ int nodes[FASTMAX_TREE_NODES], length;
+  int n = last + 1;
+  if (P.parents != nullptr) {
+    if (tid < 32) {
+      unsigned long long seen[2];
+      ancestors(P, n, tid, up, seen);
+      const unsigned long long path = __shfl_sync(0xffffffffu, last < 32 ? seen[0] : seen[1], last & 31);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if ((path >> (tid + 32 * k)) & 1ull) nodes[__popcll(path & ((1ull << (tid + 32 * k)) - 1ull))] = tid + 32 * k;
+      if (tid == 0) length = __popcll(path);
     }
-    length = n;
+    __syncthreads();
+    n = length;
   }
-  __syncthreads();
-  const int n = length;
   {
     const T* k = head_base<T>(P.k, head, P.heads);
     const T* v = head_base<T>(P.v, head, P.heads);
-    for (int idx = tid; idx < n * C4; idx += THREADS) {
-      const int i = idx / C4, c = 4 * (idx - i * C4);
-      const int node = P.parents == nullptr ? i : path[n - 1 - i];
+    for (int i = rg; i < n; i += 16) {
+      const int node = P.parents != nullptr ? nodes[i] : i;
       float x[4], y[4] = {1.f, 0.f, 0.f, 0.f};
-      if (c < D) {
+      if (c4 < D / 4) {
         Raw4<T> rk, rv;
-        rk.load(k + node * P.k.sn + c, P.aligned);
-        rv.load(v + node * P.v.sn + c, P.aligned);
+        rk.load(k + node * P.k.sn + 4 * c4, P.aligned);
+        rv.load(v + node * P.v.sn + 4 * c4, P.aligned);
         rk.get(true, x);
         rv.get(true, y);
-        *reinterpret_cast<float4*>(sK + i * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(sK + i * D + 4 * c4) = make_float4(x[0], x[1], x[2], x[3]);
       }
-      *reinterpret_cast<float4*>(sV + i * LV + c) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(sV + i * LV + 4 * c4) = make_float4(y[0], y[1], y[2], y[3]);
     }
   }
   __syncthreads();
@@ -720,7 +721,7 @@ accept_kernel(const TreeParams P, int units_each) {
     if (u < npairs) {
       const float* km = sK + 8 * ua + m8;
       const float* kn = sK + 8 * ub + n8;
-#pragma unroll 4
+#pragma unroll 2
       for (int i = 0; i < n; ++i) {
         const float4 m = *reinterpret_cast<const float4*>(km + i * D);
         const float4 y = *reinterpret_cast<const float4*>(sV + i * LV + 4 * c4);
@@ -733,6 +734,8 @@ accept_kernel(const TreeParams P, int units_each) {
       }
       if (++ub == NB) ub = ++ua;
     } else {
+      float4 ones = make_float4(0.f, 0.f, 0.f, 0.f);   // the constant's row
+      if (rg == 0) ones = __ldcs(base + (long long)(64 * npairs + D) * C4);
       for (int i = 0; i < n; ++i) {
         const float4 y = *reinterpret_cast<const float4*>(sV + i * LV + 4 * c4);
 #pragma unroll
