@@ -199,7 +199,7 @@ int32_t fastmax_decode_step(const fastmax_problem* pb, const fastmax_decode_args
 /* ---- serving: pages of moment states, and trees of drafted tokens ------------------------------------
  * A page holds one sequence's moment states, heads contiguous: head h of page p at state + p * page_stride + h * rows * ld floats
  * (rows = fastmax_state_rows, ld = fastmax_state_ld).  A model whose layers share a page passes the layer's first state and the
- * stride of whole pages.  No counterpart in the reference, which keeps nothing between two calls of its model (transformer/eval.py:8-32). */
+ * stride of whole pages.  The calls below take up to 65535 heads (batch * heads).  No counterpart in the reference, which keeps nothing between two calls of its model (transformer/eval.py:8-32). */
 typedef struct {
   float* state;         /* 16-byte aligned                                                                         */
   int64_t page_stride;  /* floats; a multiple of 4, at least heads * rows * ld where there is more than one page        */

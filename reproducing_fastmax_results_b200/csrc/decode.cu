@@ -339,8 +339,12 @@ __global__ void step_divide_kernel(const DecodeParams P, const float* parts, int
 template <typename T, int D>
 static cudaError_t launch_rows(int order, const DecodeParams& P, int bh, float* parts, cudaStream_t st) {
   const int groups = row_groups(D, order);
-  cudaError_t e = launch_after(step_rows_kernel<T, D>, dim3((unsigned)groups, (unsigned)bh), RowsGeo<D>::THREADS, 0, st, P, reinterpret_cast<float4*>(parts));
-  if (e != cudaSuccess) return e;
+  {
+    LaunchScope ls(KK_DECODE, st);
+    const cudaError_t e = launch_after(step_rows_kernel<T, D>, dim3((unsigned)groups, (unsigned)bh), RowsGeo<D>::THREADS, 0, st, P, reinterpret_cast<float4*>(parts));
+    if (e != cudaSuccess) return e;
+  }
+  LaunchScope ls(KK_DECODE, st);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((bh + 256 / D - 1) / (256 / D)));
   cfg.blockDim = dim3(D, 256 / D);
@@ -412,6 +416,7 @@ static cudaError_t launch_d(int d, int order, const DecodeParams& P, int bh, flo
       default: return launch_rows<T, 64>(order, P, bh, parts, st);
     }
   }
+  LaunchScope ls(KK_DECODE, st);
   switch (d) {
     case 16: return launch<T, 16>(order, P, bh, st);
     case 32: return launch<T, 32>(order, P, bh, st);
@@ -451,12 +456,8 @@ static int32_t decode_step(const fastmax_problem* pb, const fastmax_paged_decode
   P.c2 = pb->order == 2 ? pb->a2 * pb->inv_temperature * pb->inv_temperature : 0.f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   const int bh = pb->batch * pb->heads;
-  cudaError_t e;
-  {
-    LaunchScope ls(KK_DECODE, st);
-    e = pb->dtype == FASTMAX_BF16 ? dec::launch_d<__nv_bfloat16>(pb->d, pb->order, P, bh, parts, st)
-                                  : dec::launch_d<float>(pb->d, pb->order, P, bh, parts, st);
-  }
+  const cudaError_t e = pb->dtype == FASTMAX_BF16 ? dec::launch_d<__nv_bfloat16>(pb->d, pb->order, P, bh, parts, st)
+                                                  : dec::launch_d<float>(pb->d, pb->order, P, bh, parts, st);
   return e == cudaSuccess ? FASTMAX_OK : report_cuda_error(e);
 }
 

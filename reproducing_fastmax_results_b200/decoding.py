@@ -104,7 +104,7 @@ def per_sequence(x, like, name, low, high):
         raise ValueError(f"{name}: expected ({like.shape[0]},), got {tuple(x.shape)}")
     if not x.is_cuda and bool(((x < low) | (x > high)).any()):
         raise ValueError(f"{name}: numbers from {low} to {high} expected")
-    return x.to(device=like.device, dtype=torch.int32)
+    return _int32(x, like, low, high)
 
 
 def tree_parents(parents, like):
@@ -116,7 +116,7 @@ def tree_parents(parents, like):
         raise ValueError(f"parents: expected (b, n) for (b, h, n, d) tensors, got {tuple(parents.shape)}")
     if not parents.is_cuda and bool(((parents < -1) | (parents >= torch.arange(parents.shape[1]))).any()):
         raise ValueError("parents: every node needs a parent before it, or -1")
-    return parents.to(device=like.device, dtype=torch.int32)
+    return _int32(parents, like, -1, like.shape[2])
 
 
 def _whole(x, name):
@@ -124,3 +124,9 @@ def _whole(x, name):
     if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
         raise TypeError(f"{name}: whole numbers expected, got {x.dtype}")
     return x
+
+
+def _int32(x, like, low, high):
+    if x.is_cuda:   # what is out of range stays so when it loses its upper bits
+        x = x.clamp(low - 1, high + 1)
+    return x.to(device=like.device, dtype=torch.int32)

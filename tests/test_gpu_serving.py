@@ -497,6 +497,29 @@ def test_serving(d, order, dtype):
             assert orc.max_norm_err(got[j, :, : d + 1], ref) < (1e-5 if dtype == torch.float32 else 5e-3)
 
 
+def test_numbers_of_any_width_mean_what_they_say():
+    """64-bit numbers on the device, among them some that would be others in 32 bits; empty lists of places."""
+    from reproducing_fastmax_results_b200 import FastmaxCache
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = [torch.randn(3, 2, 4, 16, device="cuda", generator=gen) for _ in range(3)]
+    cache = FastmaxCache(3, 2, 16, temperature=10.0)
+    assert cache.begin([]).item() == 0 and cache.begin([0, 1, 2]).item() == 0
+    cache.end([])
+    cache.state[:, 0] = states(3, 2, 16, 2, gen)
+    big = 1 << 32
+    parents = torch.tensor([[-1, 0, 1, big], [-1, -1, big + 1, 0], [-1, 0, -big, 2]], device="cuda")
+    lengths = torch.tensor([4, 2, big], device="cuda")
+    o = cache.verify(*x, parents=parents, lengths=lengths)
+    ref = cache.verify(*x, parents=[[-1, 0, 1, -1], [-1, -1, -1, 0], [-1, 0, -1, 2]], lengths=[4, 2, 4])
+    assert torch.equal(o, ref) and float(o.abs().sum()) > 0
+    before = cache.state.clone()
+    cache.accept(x[1], x[2], torch.tensor([big, -big, big + 3], device="cuda"))
+    assert torch.equal(cache.state, before)
+    assert cache.arrange(torch.tensor([big, 1, -big - 2], device="cuda")).item() == 2
+    assert cache.table.tolist() == [-1, 1, -1]
+
+
 def test_the_decoder_checks_drafts():
     """FastmaxDecoder: prompt, a tree, the accepted path, the next step."""
     from reproducing_fastmax_results_b200 import FastmaxDecoder
