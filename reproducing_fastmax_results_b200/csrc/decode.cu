@@ -307,31 +307,25 @@ step_rows_kernel(const DecodeParams P, float4* parts) {
 }
 
 template <typename T, int D>
-__global__ void step_divide_kernel(const DecodeParams P, const float* parts, int groups, int total) {
-  constexpr int LD = D + 4;
+__global__ void __launch_bounds__(256)
+step_divide_kernel(const DecodeParams P, const float* parts, int groups, int total) {
+  constexpr int LD = D + 4, MOST = (Geo<D>::NPAIRS + 1 + RowsGeo<D>::EACH - 1) / RowsGeo<D>::EACH;
   grid_wait();
   grid_trigger();
   const int head = blockIdx.x * blockDim.y + threadIdx.y, c = threadIdx.x;   // a column of the state
-  __shared__ float sums[256 / D];
-  float x = 0.f, g = 0.f;
-  int bi = 0, hi = 0;
-  bool live = head < total;
-  if (live) {
-    bi = head / P.heads, hi = head - bi * P.heads;
-    live = P.table == nullptr || (P.table[bi] >= 0 && P.table[bi] < P.pages);
-  }
-  if (live) {
-    const float* at = parts + (long long)head * groups * LD;
-    for (int i = 0; i < groups; ++i) x += at[i * LD + c];
-    if (c == 0) {
-      for (int i = 0; i < groups; ++i) g += at[i * LD + D];
-      sums[threadIdx.y] = g;
-    }
-  }
-  __syncthreads();
-  if (!live) return;
+  if (head >= total) return;
+  const int bi = head / P.heads, hi = head - bi * P.heads;
+  const int page = P.table != nullptr ? P.table[bi] : 0;
+  const float* at = parts + (long long)head * groups * LD;
+  float xs[MOST], gs[MOST];   // all on their way at once; an absent sequence's are not used
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) xs[i] = i < groups ? at[i * LD + c] : 0.f, gs[i] = i < groups ? at[i * LD + D] : 0.f;
+  if (page < 0 || page >= P.pages) return;
+  float x = xs[0], g = gs[0];
+#pragma unroll
+  for (int i = 1; i < MOST; ++i) x += xs[i], g += gs[i];
   T* op = reinterpret_cast<T*>(const_cast<void*>(P.o.ptr)) + (long long)bi * P.o.sb + (long long)hi * P.o.sh;
-  op[c] = from_f<T>(x / sums[threadIdx.y]);
+  op[c] = from_f<T>(x / g);
   if (c == 0 && P.g.ptr != nullptr)
     *(reinterpret_cast<float*>(const_cast<void*>(P.g.ptr)) + (long long)bi * P.g.sb + (long long)hi * P.g.sh) = g;
 }
