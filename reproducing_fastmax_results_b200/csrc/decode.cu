@@ -459,9 +459,9 @@ extern "C" size_t fastmax_decode_step_workspace(const fastmax_problem* pb) {
   using namespace fm;
   if (!pb || pb->batch <= 0 || pb->heads <= 0 || (pb->d != 16 && pb->d != 32 && pb->d != 64) || (pb->order != 1 && pb->order != 2)) return 0;
   const long long bh = (long long)pb->batch * pb->heads;
-  // us by clusters / by short blocks: d = 64, 64 heads 19.7 / 19.7, 128 36.1 / 31.8, 512 115.7 / 106.1; d = 32, 64 heads 7.0 / 8.5, 128 12.4 / 10.2,
-  // 512 27.9 / 22.2; d = 16, 512 heads 7.3 / 8.3; order 1, d = 64, 512 heads 9.6 / 8.6.
-  if (pb->d < 32 || bh < (pb->order == 2 ? 128 : 512)) return 0;
+  // us by clusters / by short blocks: d = 64, 32 heads 12.4 / 11.1, 64 19.1 / 18.2, 96 29.7 / 24.1, 512 115.7 / 104.7; d = 32, 64 heads 6.9 / 7.3, 128
+  // 12.4 / 9.0, 512 27.9 / 21.2; d = 16, 512 heads 7.2 / 7.8, 1024 10.9 / 10.5; order 1, d = 64, 128 heads 8.1 / 3.9, 512 9.6 / 8.2.
+  if (pb->order == 2 ? bh * pb->d * pb->d < 1 << 17 : bh < 128) return 0;
   return (size_t)(bh * dec::row_groups(pb->d, pb->order) * state_ld(pb->d) * 4);
 }
 

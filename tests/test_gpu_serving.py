@@ -226,7 +226,7 @@ def test_taking_one_token_is_the_state_of_a_step(heads):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("heads", [2, 16, 19])
+@pytest.mark.parametrize("heads", [1, 2, 7])   # few heads: the dense state's own kernel, bit for bit
 def test_steps_on_pages_are_the_steps_of_a_dense_state(heads, dtype):
     from reproducing_fastmax_results_b200 import _lib as L
 
@@ -249,7 +249,8 @@ def test_steps_on_pages_are_the_steps_of_a_dense_state(heads, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("batch,heads,d,order", [(9, 16, 64, 2), (16, 8, 64, 2), (17, 8, 32, 2), (40, 13, 64, 1), (33, 16, 32, 1), (60, 16, 16, 2)])
+@pytest.mark.parametrize("batch,heads,d,order", [(9, 16, 64, 2), (4, 19, 64, 2), (17, 8, 32, 2), (40, 13, 64, 1), (9, 16, 32, 1), (60, 16, 16, 2),
+                                                   (65, 16, 16, 1)])
 def test_steps_of_many_heads_on_pages(batch, heads, d, order, dtype):
     from reproducing_fastmax_results_b200 import _lib as L
 
