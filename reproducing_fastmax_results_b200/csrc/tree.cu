@@ -158,18 +158,33 @@ __device__ __forceinline__ float* head_state(const TreeParams& P, int b, int h, 
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
-// The sums over the state are matrix products in which the state is read once for all nodes of a tree.  For one feature row-group m (the
-// rows x_m x_n, n in the blocks b >= a) the inner sums  sum_n S[(m, n)][c] x_n  are products with x itself, and  x_m  times them is added
-// in float32: nothing but the state is split into bfloat16 pieces (and x, where it is float32).
+//     o'_i = sum_r w_r Phi(q_i)_r S[r] + sum_{j in A(i)} f(q_i . k_j / T) [v_j | 1],      o_i = o'_i[:D] / o'_i[D]
+//
+// The sums over the state are matrix products in which the state is read once for all nodes of a tree.  For a row m the products x_m x_n of the
+// blocks b >= a lie one after the other, so  sum_n S[(m, n)][c] x_n  are products with x itself, and x_m times them (with the pairs' weight) is
+// added in float32: only the state is split into bfloat16 pieces, and x where it is float32.
 //
 // Layout of a product m16n8k16: 16 rows = columns c of the state, 8 columns = nodes, 16 terms = 8 + 8 rows n of two units (a, b), (a, b + 1).
+// A block has one head, or a cluster of blocks shares one; its warps divide the columns by 16 and the rows m of a unit (KG groups).  Units come
+// by the copy engine into a ring of slots; whichever warp is done last with a step asks for the units that take its place.
+//
+// Products by warps and not tcgen05: the operand that streams is the state, which has to be split on its way.  In registers it goes straight from
+// one wide load into the product; for tcgen05 its pieces would have to be written to shared memory once more, the 64 columns of a state
+// would fill half of the 128 rows, and x_m would have to be applied to tensor memory 64 times a head.
+//
+// What bounds it (bf16, 512 heads of 64 dims, order 2, 330 MB of states, 50 us at the copy rate): up to 8 nodes HBM, 53.9 us; 25 nodes 70 us and 64
+// nodes 116 us, the chain of a step (load, split, product, scale: issue slots 51 and 47 %, tensor pipe active 34 and 41 %) and the rounds of blocks:
+// 288 heads of 25 nodes take 37 us, 464 70 us, 592 72 us.  Built and left: 25 nodes, 464 heads (70 us): sixteen warps a block and one block to an SM
+// 94, two of them 91, four warps 78, three blocks of eight 90; slots 3 / 4 / 5: 85 / 71 / 70; halves of heads in clusters 79.  Copies by the
+// threads instead of the copy engine: 91 -> 71 us for 8 nodes.  Groups of products written out in turn, and cutting off instead of rounding the
+// pieces (fewer instructions), changed nothing.
 
 template <typename T>
-struct Pieces {   // of x and of the state; with two pieces of the state 2^-16 of each term is lost, with three of both 2^-24
+struct Pieces {   // of x and of the state.  bfloat16 x is one piece; two of the state keep 2^-16 of each term, far below the output's 2^-8
   static constexpr int Q = 1, S = 2;
 };
 template <>
-struct Pieces<float> {
+struct Pieces<float> {   // three of both keep 2^-24: six products
   static constexpr int Q = 3, S = 3;
 };
 
@@ -636,7 +651,9 @@ attention_kernel(const TreeParams P) {
 
 // ---- taking a path ---------------------------------------------------------------------------------------------------------
 // S[(m, n)][:] += sum over the path of k_m (k_n [v | 1]): every float of the state is read and written once.  A thread has one float4 column of four
-// rows of a unit, (m .. m + 3, n), and the next unit's four in flight meanwhile; k_n v is made once for the four.
+// rows of a unit, (m .. m + 3, n), and the next unit's four in flight meanwhile; k_n v is made once for the four.  bfloat16 k and v: exact products,
+// one rounding a token.  Short blocks of four units stream best: 512 heads of 64 dims, a path of 5: 101.7 us, the copy rate (6490 GB/s); from
+// some ten tokens on shared-memory loads bound it: 16 tokens 127 us, 64 372 us (keys kept twice to save moves: 476).
 template <int D>
 struct AcceptGeo {
   static constexpr int C4 = (D + 4) / 4;
