@@ -21,6 +21,7 @@ class FastmaxCache:
     heads, d, p, temperature, a0, a1, a2: as in `FastmaxDecoder`.  layers: attention layers whose states share a page.
     state: float32 (pages, layers, heads, rows, d + 4).  table: int32 (places,), the page of each place or -1.  Both are updated in
     place by every call, on the current stream; all calls can be captured into a CUDA graph, except those that say otherwise.
+    Nothing here records gradients; outputs must not share memory with the state, those of `verify` not with its inputs either.
     """
 
     NOTHING, EMPTY = -1, -2   # sources of `arrange` that are no places

@@ -159,6 +159,58 @@ def test_a_node_without_a_number_stays_its_own():
                 assert torch.equal(o[:, :, i], clean[:, :, i]), i
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d,n", [(16, 3), (32, 20), (64, 37)])
+def test_rows_of_any_alignment(d, n, dtype):
+    """Rows that start anywhere, at odd distances: the same bits as contiguous ones."""
+    from reproducing_fastmax_results_b200 import _lib as L
+
+    b, h = 3, 2
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    odd = [torch.randn(b, n, h, d + 3, device="cuda", generator=gen).to(dtype)[..., 1: d + 1].transpose(1, 2) for _ in range(3)]
+    even = [t.contiguous() for t in odd]
+    state = states(b, h, d, 2, gen)
+    parents = i32(random_parents(b, n, np.random.default_rng(n)))
+    wide = torch.zeros(b, h, n, d + 5, device="cuda").to(dtype)
+    o, g = L.tree_attention(*odd, state, 0.1, *A, 2, parents=parents, out=wide[..., 3: d + 3])
+    ref, gref = L.tree_attention(*even, state, 0.1, *A, 2, parents=parents)
+    assert torch.equal(o, ref) and torch.equal(g, gref)
+    assert (wide[..., :3] == 0).all() and (wide[..., d + 3:] == 0).all()
+    both = [state.clone(), state.clone()]
+    for st, (_, k, v) in zip(both, (odd, even)):
+        L.tree_accept(k, v, st, i32([n - 1, 0, n // 2]), 2, parents=parents)
+    assert torch.equal(*both)
+    table = i32([2, 0, 1])
+    outs = [L.decode_step_paged(*(t[:, :, 0] for t in x), st, table, 0.1)[0] for x, st in zip((odd, even), both)]
+    assert torch.equal(*outs) and torch.equal(*both)
+
+
+@pytest.mark.parametrize("heads", [3, 200])   # one head over a cluster of blocks, many heads
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_chain_is_that_many_steps(dtype, heads):
+    """Drafts without branches, all of them accepted: outputs and states of steps token by token, up to the rounding of either."""
+    from reproducing_fastmax_results_b200 import _lib as L
+
+    n, d = 6, 64
+    gen = torch.Generator(device="cuda").manual_seed(heads)
+    q, k, v = (torch.randn(1, heads, n, d, device="cuda", generator=gen).to(dtype) for _ in range(3))
+    stepped = states(1, heads, d, 2, gen)
+    taken = stepped.clone()
+    o, g = L.tree_attention(q, k, v, taken, 0.1, *A, 2)
+    some = [0, heads // 2, heads - 1]
+    size = [so.tree(*(host(t[0, j]) for t in (q, k, v)), host(taken[0, j]), np.arange(n) - 1, 2, A, 0.1)[2] for j in some]
+    L.tree_accept(k, v, taken, i32([n - 1]))
+    for t in range(n):
+        x, _ = L.decode_step(q[:, :, t], k[:, :, t], v[:, :, t], stepped, 0.1, *A, 2)
+        for j, s in zip(some, size):
+            a, b = host(o[0, j, t]), host(x[0, j])
+            assert (np.abs(a - b) <= so.attention_tolerance(a, s[t], dtype == torch.bfloat16) + so.attention_tolerance(b, s[t], dtype == torch.bfloat16)).all()
+    for j in some:
+        a, b = host(taken[0, j]), host(stepped[0, j])
+        _, s = so.grown(b, host(k[0, j]), host(v[0, j]), 2)
+        assert (np.abs(a - b)[:, : d + 1] <= 2 * so.grown_tolerance(s, n)).all()
+
+
 def test_an_empty_sequence_has_its_drafts_only():
     from reproducing_fastmax_results_b200 import _lib as L
 
