@@ -249,8 +249,11 @@ struct TreeGeo {
   static constexpr int N = 8 * NT;                     // nodes, filled up
   static constexpr int NB = D / 8;
   static constexpr int CG = D / 16;                    // groups of 16 columns of the state: one to a warp
-  static constexpr int BLOCKS = NT == 8 && sizeof(T) == 4 ? 1 : 2;   // to an SM
-  static constexpr int KG = D == 16 ? 8 : D == 32 || BLOCKS == 1 ? 4 : 2;   // warps that share a group and divide the rows m of a block among them
+  // Blocks to an SM, and warps that share a group of columns and divide the rows m of a unit among them: eight warps for 64 dims, four for fewer (us
+  // with eight warps, two blocks / four warps, four blocks, 512 heads: 32 dims, 8 nodes 16.2 / 11.6, 25 nodes 21.6 / 16.9; 16 dims, 16 nodes 11.6 / 7.5).
+  static constexpr bool LARGE = NT == 8 && sizeof(T) == 4;   // registers for half as many
+  static constexpr int BLOCKS = (D == 64 ? 2 : 4) / (LARGE ? 2 : 1);
+  static constexpr int KG = D == 16 || (D == 64 && LARGE) ? 4 : 2;
   static constexpr int RI = 8 / KG;
   static constexpr int WARPS = CG * KG;
   static constexpr int THREADS = 32 * WARPS;
@@ -268,7 +271,7 @@ struct TreeGeo {
   static constexpr int SUMS = KG * ROWS;
   static constexpr int FIXED = PIECES + SCALES + N * 8 + 144;
   static constexpr int SLOT = (D == 64 ? D + 1 : 64) * LDS * 4;   // a unit, or the linear rows
-  static constexpr int ROOM = (BLOCKS == 2 ? 113 : 227) * 1024 - FIXED;
+  static constexpr int ROOM = (BLOCKS == 4 ? 55 : BLOCKS == 2 ? 113 : 227) * 1024 - FIXED;
   static constexpr int SLOTS = ROOM / SLOT > 6 ? 6 : ROOM / SLOT;
   static constexpr int REGION = SLOTS * SLOT > TREE ? (SLOTS * SLOT > SUMS ? SLOTS * SLOT : SUMS) : (TREE > SUMS ? TREE : SUMS);
   static constexpr int EARLY = (REGION - TREE) / SLOT > SLOTS ? SLOTS : (REGION - TREE) / SLOT;   // slots that are free from the start
@@ -789,10 +792,10 @@ static cudaError_t launch_attention(const TreeParams& P, int bh, cudaStream_t st
   using G = TreeGeo<T, D, NT>;
   cudaError_t e = allow_bytes<attention_kernel<T, D, NT>>(G::BYTES);
   if (e != cudaSuccess) return e;
-  // A head is divided among blocks of a cluster as far as all blocks then still run at once and each has two units or more.
+  // A head is divided among blocks of a cluster as far as there are then no more than two of them for every SM, each with two units or more.
   const int units = (P.order == 2 ? Geo<D>::NPAIRS : 0) + 1;
   int cl = 1;
-  while (cl < 8 && 2LL * cl * bh <= (long long)G::BLOCKS * sm_count() && 4 * cl <= units + 1) cl *= 2;
+  while (cl < 8 && 2LL * cl * bh <= (G::BLOCKS < 2 ? 1LL : 2LL) * sm_count() && 4 * cl <= units + 1) cl *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cl, bh);
   cfg.blockDim = dim3(G::THREADS);
