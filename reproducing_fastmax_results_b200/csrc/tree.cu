@@ -59,9 +59,6 @@ struct TreeParams {
   float a0, a1, a2, inv_t;
 };
 
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-
 // four neighbours; `aligned`: all addresses are multiples of their size
 __device__ __forceinline__ void load4v(const float* p, bool aligned, float (&x)[4]) {
   if (aligned) {
@@ -176,7 +173,8 @@ __device__ __forceinline__ float* head_state(const TreeParams& P, int b, int h, 
 // nodes 116 us, the chain of a step (load, split, product, scale: issue slots 51 and 47 %, tensor pipe active 34 and 41 %) and the rounds of blocks:
 // 288 heads of 25 nodes take 37 us, 464 70 us, 592 72 us.  Built and left: 25 nodes, 464 heads (70 us): sixteen warps a block and one block to an SM
 // 94, two of them 91, four warps 78, three blocks of eight 90; slots 3 / 4 / 5: 85 / 71 / 70; halves of heads in clusters 79.  Copies by the
-// threads instead of the copy engine: 91 -> 71 us for 8 nodes.  Groups of products written out in turn, and cutting off instead of rounding the
+// threads instead of the copy engine: 91 instead of 71 us for 8 nodes at that stage.  The tree's sums as products, too: chains of 64 nodes 115
+// instead of 134 us, but trees as before and small ones 1 to 3 % slower.  Groups of products written out in turn, and cutting off instead of rounding the
 // pieces (fewer instructions), changed nothing.
 
 template <typename T>
@@ -214,7 +212,7 @@ __device__ __forceinline__ int count_up(int* counter) {   // in shared memory; o
   asm volatile("atom.add.acq_rel.cta.shared::cta.s32 %0, [%1], 1;" : "=r"(old) : "r"(smem_u32(counter)) : "memory");
   return old;
 }
-// c += s * p, the two halves of 64 bits each
+// c += s * p, two at a time
 __device__ __forceinline__ void fma2(float& c0, float& c1, float2 s, float p0, float p1) {
   asm("{\n\t.reg .b64 c, s, p;\n\t"
       "mov.b64 c, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tmov.b64 p, {%4, %5};\n\t"
@@ -294,7 +292,7 @@ attention_kernel(const TreeParams P) {
   __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem + G::REGION);           // [QP][N][LQ]: pieces of x
   float* sX = reinterpret_cast<float*>(smem + G::REGION + G::PIECES);               // [D][N]: x times the weight of the pairs, transposed
   unsigned long long* sA = reinterpret_cast<unsigned long long*>(sX + D * N);       // [N]: ancestors
-  uint64_t* full = reinterpret_cast<uint64_t*>(sA + N);                                                          // [SLOTS]: a slot's copy has arrived
+  uint64_t* full = reinterpret_cast<uint64_t*>(sA + N);                             // [SLOTS]: a slot's copy has arrived
   int* through = reinterpret_cast<int*>(full + 8);                                  // [SLOTS]: warps that are done with it
   volatile int* issued = reinterpret_cast<volatile int*>(through + 8);              // [SLOTS]: copies that were asked for
   volatile int* abort_flag = issued + 8;
