@@ -174,7 +174,8 @@ __device__ __forceinline__ float* head_state(const TreeParams& P, int b, int h, 
 // 288 heads of 25 nodes take 37 us, 464 70 us, 592 72 us.  Built and left: 25 nodes, 464 heads (70 us): sixteen warps a block and one block to an SM
 // 94, two of them 91, four warps 78, three blocks of eight 90; slots 3 / 4 / 5: 85 / 71 / 70; halves of heads in clusters 79.  Copies by the
 // threads instead of the copy engine: 91 instead of 71 us for 8 nodes at that stage.  The tree's sums as products, too: chains of 64 nodes 115
-// instead of 134 us, but trees as before and small ones 1 to 3 % slower.  Groups of products written out in turn, and cutting off instead of rounding the
+// instead of 134 us, but trees as before and small ones 1 to 3 % slower.  The last units of rows of odd length paired up with m and n exchanged (18
+// steps instead of 20, the units out of their order): 77.  Groups of products written out in turn, and cutting off instead of rounding the
 // pieces (fewer instructions), changed nothing.
 
 template <typename T>
