@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .attention import _ext
-from .decoding import per_sequence, tree_parents
+from .decoding import check_prompts, per_sequence, tree_parents
 
 
 class FastmaxCache:
@@ -81,10 +81,10 @@ class FastmaxCache:
         """Causal attention of prompts, (len(places), h, n, d), whose sequences are in `places` (different numbers on the host; they have
         their pages).  The layer's states are replaced by the prompts', or with `continues` extended.  Returns o.  Not for capture."""
         places = self._distinct(places)
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            if t.dim() != 4 or t.shape[0] != len(places) or t.shape[1] != self.heads or t.shape[3] != self.d or t.shape[2] != q.shape[2]:
-                raise ValueError(f"{name}: expected ({len(places)}, {self.heads}, n, {self.d}), got {tuple(t.shape)}")
         states = self._layer(layer)
+        check_prompts(q, k, v, len(places), states)
+        if not places:
+            return q.new_empty(q.shape)
         index = self.table[torch.tensor(places, device=self.table.device)]
         before = None
         if continues:

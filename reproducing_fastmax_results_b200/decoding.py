@@ -90,6 +90,24 @@ class FastmaxDecoder:
         self.tokens_seen += k.shape[2]
 
 
+def check_prompts(q, k, v, batch, state):
+    """Prompts' q, k, v for the `batch` sequences of `state` (float32 (..., heads, rows, d + 4)): all of it is refused here, before anything is
+    launched, since the binding that prompts go through takes the sizes, the type and the device of all three from q."""
+    heads, d = state.shape[-3], state.shape[-1] - 4
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4 or tuple(t.shape) != (batch, heads, q.shape[2], d):
+            raise ValueError(f"{name}: expected ({batch}, {heads}, n, {d}), got {tuple(t.shape)}")
+    if q.shape[2] == 0:
+        raise ValueError("a prompt needs a token")
+    _lib.dtype_code(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError(f"dtypes differ: q {q.dtype}, k {k.dtype}, v {v.dtype}")
+    if any(t.stride(3) != 1 for t in (q, k, v)):
+        raise RuntimeError("the head dim must be contiguous")
+    if any(not t.is_cuda or t.device != state.device for t in (q, k, v)):
+        raise RuntimeError(f"q, k, v must be CUDA tensors on the state's device {state.device}, got {q.device}, {k.device}, {v.device}")
+
+
 def _is_there(x):
     return x is None or (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.int32)
 

@@ -550,6 +550,30 @@ def test_serving(d, order, dtype):
             assert orc.max_norm_err(got[j, :, : d + 1], ref) < (1e-5 if dtype == torch.float32 else 5e-3)
 
 
+def test_prompts_of_mixed_types_and_devices_are_refused():
+    """Before anything is launched: the states stay as they are, and the next prompt is right.  No places: no prompts."""
+    from reproducing_fastmax_results_b200 import FastmaxCache
+
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = [torch.randn(2, 2, 9, 32, device="cuda", generator=gen) for _ in range(3)]
+    cache = FastmaxCache(3, 2, 32, temperature=10.0)
+    assert cache.begin([0, 1, 2]).item() == 0
+    cache.state[:, 0] = states(3, 2, 32, 2, gen)
+    before = cache.state.clone()
+    for i in range(3):
+        for other in (x[i].bfloat16(), x[i].cpu(), x[i].transpose(2, 3).contiguous().transpose(2, 3)):
+            bad = [other if j == i else t for j, t in enumerate(x)]
+            for continues in (False, True):
+                with pytest.raises(RuntimeError):
+                    cache.prefill(*bad, [0, 2], continues=continues)
+    none = [t[:0] for t in x]
+    assert tuple(cache.prefill(*none, []).shape) == (0, 2, 9, 32)
+    assert torch.equal(cache.state, before)
+    o = cache.prefill(*x, [0, 2])
+    assert orc.max_norm_err(host(o), causal(*x, 0.1)) < 1e-4
+    assert torch.equal(cache.state[1], before[1]) and not torch.equal(cache.state[0], before[0])
+
+
 def test_numbers_of_any_width_mean_what_they_say():
     """64-bit numbers on the device, among them some that would be others in 32 bits; empty lists of places."""
     from reproducing_fastmax_results_b200 import FastmaxCache

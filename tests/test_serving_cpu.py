@@ -159,6 +159,38 @@ def test_caches_that_cannot_be_are_refused():
         cache.verify(x, x, x)
 
 
+def test_prompts_on_pages_are_checked_before_any_launch(monkeypatch):
+    """One type, one device and unit strides for q, k and v: the binding behind takes all three from q."""
+    from reproducing_fastmax_results_b200 import FastmaxCache, cache as module
+
+    def reached(*args, **options):
+        raise AssertionError("the prompt was launched")
+
+    monkeypatch.setattr(module._lib, "forward", reached)
+    monkeypatch.setattr(module, "_ext", reached)
+    cache = FastmaxCache(3, 2, 16, layers=2, device="cpu")
+    x, y = torch.zeros(2, 2, 4, 16), torch.zeros(2, 2, 4, 16, dtype=torch.bfloat16)
+    apart = torch.zeros(2, 2, 16, 4).transpose(2, 3)
+    for continues in (False, True):
+        for q, k, v in ((x, y, x), (x, x, y), (y, x, x), (x, y, y), (y, y, x)):
+            with pytest.raises(RuntimeError, match="dtypes differ"):
+                cache.prefill(q, k, v, [0, 2], layer=1, continues=continues)
+        for q, k, v in ((apart, x, x), (x, apart, x), (x, x, apart)):
+            with pytest.raises(RuntimeError, match="contiguous"):
+                cache.prefill(q, k, v, [0, 2], continues=continues)
+        for bad in (x.half(), x.double(), x.int()):
+            with pytest.raises(TypeError):
+                cache.prefill(bad, bad, bad, [0, 2], continues=continues)
+        for q, k, v in ((x, x, x), (y, y, y)):   # on the host
+            with pytest.raises(RuntimeError, match="CUDA"):
+                cache.prefill(q, k, v, [0, 2], continues=continues)
+        for q, k, v in ((x[:, :, :0],) * 3, (x[0],) * 3, (x, x, x[:, :, :3]), (x, x[:, :1], x), (x, x, x[..., :8])):
+            with pytest.raises(ValueError):
+                cache.prefill(q, k, v, [0, 2], continues=continues)
+    with pytest.raises(ValueError):
+        cache.prefill(x, x, x, [0, 1], layer=2)
+
+
 # ---- the oracle ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("order", [1, 2])
 @pytest.mark.parametrize("d", [16, 32])
