@@ -55,13 +55,11 @@ class FastmaxDecoder:
     def prefill(self, q, k, v):
         """Causal attention of a (b, h, n, d) block that continues the sequence seen so far.  Returns o (b, h, n, d)
         and adds the block's keys and values to the state."""
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            self._check(t, name)
-        if q.dim() != 4 or q.shape[2] != k.shape[2]:
-            raise ValueError("prefill takes (b, h, n, d) tensors with as many queries as keys")
-        o, _, state = _lib.forward(q, k, v, True, self.inv_temperature, self.a0, self.a1, self.a2, self.p,
-                                   state_in=self.state if self.tokens_seen else None, want_state=True,
-                                   flags=_lib.FLAG_PAIRWISE)
+        check_prompts(q, k, v, self.batch, self.state)
+        with torch.cuda.device(self.state.device):
+            o, _, state = _lib.forward(q, k, v, True, self.inv_temperature, self.a0, self.a1, self.a2, self.p,
+                                       state_in=self.state if self.tokens_seen else None, want_state=True,
+                                       flags=_lib.FLAG_PAIRWISE)
         self.state = state
         self.tokens_seen += q.shape[2]
         return o

@@ -191,6 +191,31 @@ def test_prompts_on_pages_are_checked_before_any_launch(monkeypatch):
         cache.prefill(x, x, x, [0, 1], layer=2)
 
 
+def test_prompts_of_the_decoder_are_checked_before_any_launch(monkeypatch):
+    """As on pages; a v shorter than k would be read past its end."""
+    from reproducing_fastmax_results_b200 import FastmaxDecoder, decoding as module
+
+    def reached(*args, **options):
+        raise AssertionError("the prompt was launched")
+
+    monkeypatch.setattr(module._lib, "forward", reached)
+    dec = FastmaxDecoder(2, 3, 16, device="cpu")
+    x, y = torch.zeros(2, 3, 4, 16), torch.zeros(2, 3, 4, 16, dtype=torch.bfloat16)
+    for q, k, v in ((x, x, x[:, :, :3]), (x, x[:, :, :3], x), (x[0], x, x), (x, x, x[0]), (x, x[:1], x), (x, x, x[..., :8]), (x[:, :, :0],) * 3):
+        with pytest.raises(ValueError):
+            dec.prefill(q, k, v)
+    for q, k, v in ((x, y, x), (x, x, y), (y, x, y)):
+        with pytest.raises(RuntimeError, match="dtypes differ"):
+            dec.prefill(q, k, v)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        dec.prefill(x, x, torch.zeros(2, 3, 16, 4).transpose(2, 3))
+    with pytest.raises(TypeError):
+        dec.prefill(x.half(), x.half(), x.half())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        dec.prefill(x, x, x)
+    assert dec.tokens_seen == 0
+
+
 # ---- the oracle ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("order", [1, 2])
 @pytest.mark.parametrize("d", [16, 32])
