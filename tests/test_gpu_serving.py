@@ -574,6 +574,21 @@ def test_prompts_of_mixed_types_and_devices_are_refused():
     assert torch.equal(cache.state[1], before[1]) and not torch.equal(cache.state[0], before[0])
 
 
+def test_a_step_into_memory_of_another_device_is_refused():
+    """Before the launch, with a dense state and on pages."""
+    from reproducing_fastmax_results_b200 import FastmaxCache, FastmaxDecoder
+
+    x = [torch.ones(2, 2, 16, device="cuda") for _ in range(3)]
+    dec, cache = FastmaxDecoder(2, 2, 16), FastmaxCache(2, 2, 16)
+    cache.begin([0, 1])
+    for serve in (dec, cache):
+        with pytest.raises(RuntimeError, match="device"):
+            serve.step(*x, out=torch.zeros(2, 2, 16))
+        assert (serve.state == 0).all()
+    assert dec.tokens_seen == 0
+    assert torch.equal(dec.step(*x), cache.step(*x))
+
+
 def test_numbers_of_any_width_mean_what_they_say():
     """64-bit numbers on the device, among them some that would be others in 32 bits; empty lists of places."""
     from reproducing_fastmax_results_b200 import FastmaxCache
