@@ -137,9 +137,9 @@ def tree_parents(parents, like):
 
 def _whole(x, name):
     x = torch.as_tensor(x)
-    if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
-        raise TypeError(f"{name}: whole numbers expected, got {x.dtype}")
-    return x
+    if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype in (torch.bool, torch.uint64):   # uint64: not all of it fits below
+        raise TypeError(f"{name}: whole numbers of up to 64 bits with a sign expected, got {x.dtype}")
+    return x.to(torch.int64)   # bounds are compared in 64 bits: a narrow type does not hold them all
 
 
 def _int32(x, like, low, high):

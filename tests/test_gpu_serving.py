@@ -612,6 +612,36 @@ def test_numbers_of_any_width_mean_what_they_say():
     assert cache.table.tolist() == [-1, 1, -1]
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int64])
+def test_device_numbers_of_narrow_types_are_what_they_say(dtype):
+    """lengths, last, parents and sources in types that do not hold the bounds they are compared with."""
+    from reproducing_fastmax_results_b200 import FastmaxCache
+
+    def narrow(x):
+        return torch.tensor(x, dtype=dtype, device="cuda")
+
+    signed = dtype != torch.uint8
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = [torch.randn(200, 1, 4, 16, device="cuda", generator=gen) for _ in range(3)]
+    start = states(200, 1, 16, 2, gen)
+    caches = [FastmaxCache(200, 1, 16, temperature=10.0) for _ in range(2)]
+    for cache in caches:
+        assert cache.begin(range(200)).item() == 0
+        cache.state[:, 0] = start
+    lengths, last = [i % 5 for i in range(200)], [i % 4 for i in range(200)]
+    parents = [[-1 if signed else 0, 0, 1, 1 - i % 2] for i in range(200)]
+    roots = [[-1, *row[1:]] for row in parents]   # an unsigned 0 at the first node is no node before it: a root
+    sources = [min(199 - i, 127) for i in range(200)]   # int8 holds them
+    o = caches[0].verify(*x, parents=narrow(parents), lengths=narrow(lengths))
+    ref = caches[1].verify(*x, parents=i32(roots), lengths=i32(lengths))
+    assert torch.equal(o, ref) and (o[4] != 0).any() and (o[5] == 0).all()
+    caches[0].accept(x[1], x[2], narrow(last), parents=narrow(parents))
+    caches[1].accept(x[1], x[2], i32(last), parents=i32(roots))
+    assert torch.equal(caches[0].state, caches[1].state) and not torch.equal(caches[0].state[:, 0], start)
+    assert caches[0].arrange(narrow(sources)).tolist() == caches[1].arrange(i32(sources)).tolist() == [0]
+    assert torch.equal(caches[0].table, caches[1].table) and torch.equal(caches[0].state, caches[1].state)
+
+
 def test_the_decoder_checks_drafts():
     """FastmaxDecoder: prompt, a tree, the accepted path, the next step."""
     from reproducing_fastmax_results_b200 import FastmaxDecoder

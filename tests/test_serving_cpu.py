@@ -140,6 +140,29 @@ def test_numbers_on_the_host_are_checked():
         tree_parents(good, like[:, 0])
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64])
+def test_host_numbers_of_narrow_types_are_what_they_say(dtype):
+    signed = dtype not in (torch.uint8, torch.uint16, torch.uint32)
+    like = torch.zeros(3, 2, 4, 16)
+    wide = torch.zeros(200, 1, 1, 16)
+    top = min(199, torch.iinfo(dtype).max)
+    for numbers, low, high in (([3, 0, 1], -1, 3), ([4, 0, 2], 0, 4), ([0, 2, 1], -2, 2)):
+        got = per_sequence(torch.tensor(numbers, dtype=dtype), like, "x", low, high)
+        assert got.dtype == torch.int32 and got.tolist() == numbers
+    got = per_sequence(torch.full((200,), top, dtype=dtype), wide, "x", -2, 199)
+    assert got.tolist() == [top] * 200
+    rows = [[-1 if signed else 0, 0, 1, 2]] * 3
+    if signed:
+        assert tree_parents(torch.tensor(rows, dtype=dtype), like).tolist() == rows
+    else:   # a root cannot be said in a type without a sign
+        with pytest.raises(ValueError):
+            tree_parents(torch.tensor(rows, dtype=dtype), like)
+    with pytest.raises(ValueError):
+        per_sequence(torch.tensor([5, 0, 0], dtype=dtype), like, "x", -1, 4)
+    with pytest.raises(TypeError):
+        per_sequence(torch.tensor([5, 0, 0], dtype=torch.uint64), like, "x", -1, 9)
+
+
 def test_caches_that_cannot_be_are_refused():
     from reproducing_fastmax_results_b200 import FastmaxCache
 
