@@ -342,7 +342,7 @@ const char* fastmax_version(void);
  * Call it after synchronising the stream.  No counterpart in the reference (it never checks its launches). */
 int32_t fastmax_check_status(void);
 /* Diagnostics for FASTMAX_ERR_DEVICE_TIMEOUT: out[i] = how many thread blocks gave up first at wait site i
- * (i = the site's code modulo 256; the codes are listed beside the waits in csrc/tc_*.cuh).  Synchronous; clears
+ * (i = the site's code modulo 256; the codes are listed beside the waits in csrc/).  Synchronous; clears
  * the counters.  No counterpart in the reference. */
 int32_t fastmax_debug_wait_histogram(int32_t* out, int32_t n);
 /* Exercises the failure path of the bounded device-side waits without touching a production kernel: launches one
@@ -351,6 +351,9 @@ int32_t fastmax_debug_wait_histogram(int32_t* out, int32_t n);
  * FASTMAX_ERR_DEVICE_TIMEOUT once (then FASTMAX_OK again) and fastmax_debug_wait_histogram() shows one block at
  * wait site 99.  The context stays usable; nothing faults, traps or hangs.  No counterpart in the reference. */
 int32_t fastmax_debug_wait_selftest(void* cuda_stream);
+/* The same for the waits of fastmax_tree_attention, at wait site 210: a thread block whose copy never comes gives up, waits for the copy
+ * that it has in flight and returns. */
+int32_t fastmax_debug_tree_wait_selftest(void* cuda_stream);
 /* Number of kernel launches issued by this library in this process (all entry points, all threads). */
 uint64_t fastmax_launch_count(void);
 

@@ -28,7 +28,7 @@ EXPORTED_SYMBOLS = [
     "fastmax_key_prologue", "fastmax_output_noise",
     "fastmax_status_string", "fastmax_last_cuda_error", "fastmax_last_cuda_error_string",
     "fastmax_version", "fastmax_launch_count", "fastmax_check_status", "fastmax_debug_wait_histogram",
-    "fastmax_debug_wait_selftest",
+    "fastmax_debug_wait_selftest", "fastmax_debug_tree_wait_selftest",
     "fastmax_profile_enable", "fastmax_profile_kinds", "fastmax_profile_kind_name", "fastmax_profile_collect",
 ]
 
@@ -189,6 +189,8 @@ def load():
     lib.fastmax_debug_wait_histogram.argtypes = [C.POINTER(C.c_int32), C.c_int32]
     lib.fastmax_debug_wait_selftest.restype = C.c_int32
     lib.fastmax_debug_wait_selftest.argtypes = [C.c_void_p]
+    lib.fastmax_debug_tree_wait_selftest.restype = C.c_int32
+    lib.fastmax_debug_tree_wait_selftest.argtypes = [C.c_void_p]
     lib.fastmax_profile_enable.argtypes = [C.c_int32]
     lib.fastmax_profile_kind_name.restype = C.c_char_p
     lib.fastmax_profile_kind_name.argtypes = [C.c_int32]

@@ -28,21 +28,61 @@ __device__ int g_status = 0;       // see tc_device_status
 __device__ int g_wait_hist[256];
 
 constexpr long long WAIT_CYCLES = 4000000000ll;   // ~2 s at 2 GHz
+constexpr int WAIT_SLOT = 210;                    // the site's code: a slot of the state
 
 // Waits for the phase of parity `parity`.  Returns in any case: when the wait runs out (code `code`), the flag is up, no further copy is
-// asked for and every later wait of the block falls through at once.
+// asked for and every later wait of the block falls through at once.  The thread that raises the flag reports, so a block counts once.
+template <long long LIMIT = WAIT_CYCLES>
 __device__ __noinline__ void wait_slow(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
-  if (*abort_flag == 0 && !mbar_wait_abortable(bar, parity, WAIT_CYCLES, abort_flag)) {
-    if (*abort_flag == 0) atomicAdd(&g_wait_hist[code & 255], 1);
-    *abort_flag = 1;
+  if (*abort_flag == 0 && !mbar_wait_abortable(bar, parity, LIMIT, abort_flag) && atomicExch(const_cast<int*>(abort_flag), 1) == 0) {
+    atomicAdd(&g_wait_hist[code & 255], 1);
     atomicExch(&g_status, code);
   }
 }
+template <long long LIMIT = WAIT_CYCLES>
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
   // (a test that does not suspend the thread: waking it costs some 250 clocks, and the copy has mostly arrived)
   for (int i = 0; i < 64; ++i)
     if (mbar_test_wait(bar, parity)) return;
-  wait_slow(bar, parity, code, abort_flag);
+  wait_slow<LIMIT>(bar, parity, code, abort_flag);
+}
+// Behind a block's last wait and a barrier, called by all threads where a wait ran out: nobody writes into the slots or leaves while a copy is
+// under way.
+__device__ __noinline__ void drain(uint64_t* full, const volatile int* issued, int slots) {
+  if (threadIdx.x == 0)
+    for (int i = 0; i < slots; ++i)
+      if (issued[i] > 0) mbar_wait_bounded(&full[i], (uint32_t)(issued[i] - 1) & 1u, WAIT_CYCLES);
+  __syncthreads();
+}
+
+// What a block does that gives up, without a state: one slot's copy never comes (nobody asks for it), the other's is under way meanwhile.
+// A slot that the drain leaves before its copy is there counts at the site behind.
+constexpr int SELFTEST_FLOATS = 64;
+__device__ __align__(16) float g_selftest_source[SELFTEST_FLOATS];   // zeros
+__global__ void wait_selftest_kernel() {
+  __shared__ __align__(128) float slot[SELFTEST_FLOATS];
+  __shared__ uint64_t full[2];
+  __shared__ int flags[3];
+  volatile int* issued = flags;
+  volatile int* abort_flag = flags + 2;
+  const int tid = threadIdx.x;
+  slot[tid] = 1.f;
+  if (tid == 0) {
+    mbar_init(&full[0], 1), mbar_init(&full[1], 1);
+    issued[0] = 0, issued[1] = 1, *abort_flag = 0;
+    fence_mbar_init();
+  }
+  fence_proxy_async_smem();
+  __syncthreads();
+  if (tid == 0) {
+    mbar_arrive_expect_tx(&full[1], sizeof(slot));
+    bulk_load(slot, g_selftest_source, sizeof(slot), &full[1]);
+  }
+  wait<2000000ll>(&full[0], 0u, WAIT_SLOT, abort_flag);   // about a millisecond
+  wait(&full[0], 0u, WAIT_SLOT, abort_flag);              // falls through
+  __syncthreads();
+  if (*abort_flag != 0) drain(full, issued, 2);
+  if (slot[tid] != 0.f) atomicAdd(&g_wait_hist[WAIT_SLOT + 1], 1);
 }
 
 struct TreeParams {
@@ -548,7 +588,7 @@ attention_kernel(const TreeParams P) {
   };
   int done = 0;   // units
   auto unit = [&](int i) -> const float* {
-    wait(&full[i % SLOTS], (uint32_t)(i / SLOTS) & 1u, 210, abort_flag);
+    wait(&full[i % SLOTS], (uint32_t)(i / SLOTS) & 1u, WAIT_SLOT, abort_flag);
     return reinterpret_cast<const float*>(smem + (i % SLOTS) * G::SLOT);
   };
   // the last warp that is done with a step asks for the units that take its slots
@@ -612,9 +652,7 @@ attention_kernel(const TreeParams P) {
     }
   }
   __syncthreads();   // nobody reads the state any more
-  if (tid == 0 && *abort_flag != 0)   // leave only after the copies in flight
-    for (int i = 0; i < SLOTS; ++i)
-      if (issued[i] > 0) mbar_wait_bounded(&full[i], (uint32_t)(issued[i] - 1) & 1u, WAIT_CYCLES);
+  if (*abort_flag != 0) drain(full, issued, SLOTS);
   // ---- partial sums meet, the warps' and the cluster's blocks', in a fixed order ------------------------------------------------
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -895,6 +933,13 @@ int tree_wait_histogram(int* out, int n) {
 }
 
 }  // namespace fm
+
+extern "C" int32_t fastmax_debug_tree_wait_selftest(void* cuda_stream) {
+  using namespace fm;
+  tree::wait_selftest_kernel<<<1, tree::SELFTEST_FLOATS, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>();
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? FASTMAX_OK : report_cuda_error(e);
+}
 
 extern "C" int32_t fastmax_tree_attention(const fastmax_problem* pb, const fastmax_tree_args* a, void* cuda_stream) {
   using namespace fm;

@@ -753,6 +753,34 @@ def test_calls_on_two_streams_keep_apart():
         assert all(torch.equal(a, b) for a, b in zip(outs, ref))
 
 
+def test_a_tree_that_gives_up_is_reported_once_and_the_context_stays_usable():
+    """The waits of the tree's kernel: a block whose copy never comes ends by itself after about a millisecond, waits for its other copy, and counts
+    as one block at its wait site.  No operator is disturbed."""
+    from reproducing_fastmax_results_b200 import _lib as L
+
+    lib = L.load()
+    torch.cuda.synchronize()
+    assert lib.fastmax_check_status() == 0 and L.wait_histogram() == {}
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.fastmax_debug_tree_wait_selftest(stream) == 0
+    torch.cuda.synchronize()
+    assert lib.fastmax_check_status() == 5 and lib.fastmax_check_status() == 0   # FASTMAX_ERR_DEVICE_TIMEOUT, once
+    assert L.wait_histogram() == {210: 1} and L.wait_histogram() == {}
+    # beside another kernel's
+    assert lib.fastmax_debug_wait_selftest(stream) == 0 and lib.fastmax_debug_tree_wait_selftest(stream) == 0
+    with pytest.raises(L.FastmaxError):
+        L.check_status()
+    assert lib.fastmax_check_status() == 0
+    assert L.wait_histogram() == {99: 1, 210: 1} and L.wait_histogram() == {}
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(1, 2, 20, 64, device="cuda", generator=gen) for _ in range(3))
+    state = states(1, 2, 64, 2, gen)
+    o, g = L.tree_attention(q, k, v, state, 0.1, *A, 2)
+    check_tree(o, g, q, k, v, state, None, None, None, 2, 0.1)
+    L.check_status()
+    assert L.wait_histogram() == {}
+
+
 def test_calls_back_to_back_see_each_other():
     """A kernel starts while the one before it ends: a chain of dependent calls gives the same as with a wait behind each."""
     from reproducing_fastmax_results_b200 import FastmaxCache
