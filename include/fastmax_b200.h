@@ -206,7 +206,8 @@ typedef struct {
   int32_t pages;        /* pages that exist                                                                             */
   int32_t reserved;
   const int32_t* table; /* [batch]: the page of each sequence, each page at most once; an entry outside 0 .. pages-1 says that the   */
-                        /* sequence is absent: nothing of it is read or written.  NULL: sequence b has page b (pages >= batch)  */
+                        /* sequence is absent: no state is read or written for it, and its outputs stay as they were.  Its part of  */
+                        /* the other arguments must be readable all the same.  NULL: sequence b has page b (pages >= batch)     */
 } fastmax_pages;
 
 /* fastmax_decode_step with a page per sequence.  The outputs of absent sequences stay as they were.  workspace:
@@ -229,6 +230,8 @@ int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged
  *       follows the cached sequence directly.  Any other value counts as -1.  NULL: every node follows the one before it.
  *   lengths (optional): int32 [batch], nodes of each sequence (0 .. nq; outside of that range it counts as the nearer end).
  *       Rows behind it, and all rows of absent sequences, are not written.
+ *   q, k, v: all nq rows of every sequence must be readable, whatever table and lengths say: they are asked for before it is known which
+ *       of them count.  What stands in rows that do not count changes nothing.
  *   o must not share memory with q, k, v or the state. */
 #define FASTMAX_TREE_NODES 64
 typedef struct {

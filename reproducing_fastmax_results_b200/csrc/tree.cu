@@ -355,8 +355,8 @@ attention_kernel(const TreeParams P) {
   };
   grid_wait();
   grid_trigger();
-  // Queries, keys and values of all rows that the tensors have are asked for at once, before it is known which of them count: what comes
-  // behind the copies of the state waits for those.
+  // Queries, keys and values of all rows that the tensors have (the caller sees to it that they are readable) are asked for at once, before it
+  // is known which of them count: what comes behind the copies of the state waits for those.
   constexpr int ITEMS = (N * (D / 4) + THREADS - 1) / THREADS;
   Raw4<T> rq[ITEMS], rk[ITEMS], rv[ITEMS];
   {
