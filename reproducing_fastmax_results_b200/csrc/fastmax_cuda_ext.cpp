@@ -7,6 +7,7 @@
 // the denominator in the last column), plus strided/bf16 entry points used by the FastMax autograd Function.
 // torch is used for memory (outputs, workspace from the caching allocator), the device guard and the
 // current stream; all arithmetic happens in the library's own kernels.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -504,6 +505,7 @@ torch::Tensor fastmax_op(torch::Tensor q, torch::Tensor k, torch::Tensor v, bool
 // one token per (batch, head) against the carried state: q, k, v (b, h, d) or (b, h, 1, d); returns o shaped like q
 torch::Tensor decode_step(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor state, double inv_temp, double a0, double a1,
                           double a2, int64_t p, c10::optional<torch::Tensor> out) {
+  if (out.has_value() && out->defined()) at::assert_no_internal_overlap(*out);
   CHECK_CUDA(q); CHECK_CUDA(k); CHECK_CUDA(v); CHECK_CUDA(state);
   TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q, k, v must be (b, h, d) or (b, h, 1, d)");
   TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k, v dtypes differ");
@@ -534,6 +536,11 @@ torch::Tensor decode_step(torch::Tensor q, torch::Tensor k, torch::Tensor v, tor
 // ---- serving: pages of moment states, trees of drafted tokens --------------------------------------------------------
 using maybe = c10::optional<torch::Tensor>;
 bool given(const maybe& t) { return t.has_value() && t->defined(); }
+// the caller's output: rows that lie on one another (an expanded tensor) would be written at once
+bool given_output(const maybe& out) {
+  if (given(out)) at::assert_no_internal_overlap(*out);
+  return given(out);
+}
 
 // Shapes are checked here, before anything else and as ValueError: the Python classes pass their arguments straight on.
 // state: float32 (pages, heads, rows, ld), pages any distance apart (a layer of a cache); table: int32 (batch,) or none
@@ -593,8 +600,8 @@ torch::Tensor parents_rows(const maybe& parents) {
 
 torch::Tensor tree_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& state, const maybe& table,
                              const maybe& parents, const maybe& lengths, double inv_temp, double a0, double a1, double a2, int64_t p, const maybe& out) {
-  fastmax_problem pb = given(out) ? tree_problem({&q, &k, &v, &*out}, state, table, p, &parents, given(lengths) ? &*lengths : nullptr)
-                                  : tree_problem({&q, &k, &v}, state, table, p, &parents, given(lengths) ? &*lengths : nullptr);
+  fastmax_problem pb = given_output(out) ? tree_problem({&q, &k, &v, &*out}, state, table, p, &parents, given(lengths) ? &*lengths : nullptr)
+                                         : tree_problem({&q, &k, &v}, state, table, p, &parents, given(lengths) ? &*lengths : nullptr);
   pb.a0 = (float)a0; pb.a1 = (float)a1; pb.a2 = (float)a2; pb.inv_temperature = (float)inv_temp;
   const c10::cuda::CUDAGuard guard(q.device());
   fastmax_tree_args a{};
@@ -627,7 +634,7 @@ void tree_accept(const torch::Tensor& k, const torch::Tensor& v, const torch::Te
 torch::Tensor decode_step_paged(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& state,
                                 const torch::Tensor& table, double inv_temp, double a0, double a1, double a2, int64_t p, const maybe& out) {
   auto rows = [](const torch::Tensor& t) { return t.dim() == 3 ? t.unsqueeze(2) : t; };
-  const torch::Tensor q4 = rows(q), k4 = rows(k), v4 = rows(v), given_out = given(out) ? rows(*out) : torch::Tensor();
+  const torch::Tensor q4 = rows(q), k4 = rows(k), v4 = rows(v), given_out = given_output(out) ? rows(*out) : torch::Tensor();
   fastmax_problem pb = given_out.defined() ? tree_problem({&q4, &k4, &v4, &given_out}, state, table, p) : tree_problem({&q4, &k4, &v4}, state, table, p);
   TORCH_CHECK_VALUE(pb.nq == 1, "one token per (batch, head) expected, got ", q.sizes());
   pb.a0 = (float)a0; pb.a1 = (float)a1; pb.a2 = (float)a2; pb.inv_temperature = (float)inv_temp;

@@ -239,6 +239,21 @@ def test_prompts_of_the_decoder_are_checked_before_any_launch(monkeypatch):
     assert dec.tokens_seen == 0
 
 
+def test_outputs_whose_rows_lie_on_one_another_are_refused():
+    from reproducing_fastmax_results_b200 import FastmaxCache, FastmaxDecoder
+
+    x = torch.zeros(3, 2, 4, 16)
+    cache, dec = FastmaxCache(3, 2, 16, device="cpu"), FastmaxDecoder(3, 2, 16, device="cpu")
+    for out in (torch.zeros(1, 2, 4, 16), torch.zeros(3, 1, 4, 16), torch.zeros(3, 2, 1, 16), torch.zeros(1)):
+        for serve in (cache, dec):
+            with pytest.raises(RuntimeError, match="single memory location"):
+                serve.verify(x, x, x, out=out.expand(3, 2, 4, 16))
+    for out in (torch.zeros(1, 2, 16), torch.zeros(3, 1, 16), torch.zeros(1)):
+        for serve in (cache, dec):
+            with pytest.raises(RuntimeError, match="single memory location"):
+                serve.step(x[:, :, 0], x[:, :, 0], x[:, :, 0], out=out.expand(3, 2, 16))
+
+
 # ---- the oracle ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("order", [1, 2])
 @pytest.mark.parametrize("d", [16, 32])
