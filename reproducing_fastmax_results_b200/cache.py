@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .attention import _ext
-from .decoding import check_prompts, per_sequence, tree_parents
+from .decoding import check_prompts, per_sequence, refuse_capture, tree_parents
 
 
 class FastmaxCache:
@@ -20,7 +20,9 @@ class FastmaxCache:
 
     heads, d, p, temperature, a0, a1, a2: as in `FastmaxDecoder`.  layers: attention layers whose states share a page.
     state: float32 (pages, layers, heads, rows, d + 4).  table: int32 (places,), the page of each place or -1.  Both are updated in
-    place by every call, on the current stream; all calls can be captured into a CUDA graph, except those that say otherwise.
+    place by every call, on the current stream.  With sources, parents, lengths and last on the device no call waits for it, and all of them
+    can be captured into a CUDA graph; numbers on the host (lists, tensors there; `begin`, `end` and `prefill` have them always) are copied
+    first, for which the call waits, and are refused during a capture.
     Nothing here records gradients; outputs must not share memory with the state, those of `verify` not with its inputs either.
     """
 
@@ -49,11 +51,12 @@ class FastmaxCache:
         return _ext().cache_arrange(self.state, self.table, per_sequence(sources, self.table, "sources", -2, self.places - 1))
 
     def begin(self, places):
-        """Starts an empty sequence in each of these places (numbers on the host), whatever they held.  Returns what arrange returns."""
+        """Starts an empty sequence in each of these places (numbers on the host: not for capture), whatever they held.  Returns what arrange
+        returns."""
         return self.arrange(self._with(places, self.EMPTY))
 
     def end(self, places):
-        """Frees the pages of these places (numbers on the host)."""
+        """Frees the pages of these places (numbers on the host: not for capture)."""
         self.arrange(self._with(places, self.NOTHING))
 
     def _distinct(self, places):
@@ -85,6 +88,7 @@ class FastmaxCache:
         check_prompts(q, k, v, len(places), states)
         if not places:
             return q.new_empty(q.shape)
+        refuse_capture(q.device)
         index = self.table[torch.tensor(places, device=self.table.device)]
         before = None
         if continues:

@@ -77,13 +77,14 @@ class FastmaxDecoder:
         """Attention of drafted tokens, (b, h, n, d) with n <= 64, that leaves the state as it is: node i sees the sequence so far, its
         ancestors and itself.  parents: int32 (b, n), the parent of each node (a node before it, or -1: the sequence itself); None: a chain.
         lengths: int32 (b,), nodes of each sequence.  Returns o (b, h, n, d); rows behind a sequence's nodes stay as they are in
-        `out`, zero without one."""
+        `out`, zero without one.  Can be captured into a CUDA graph with parents and lengths on the device."""
         return _ext().tree_attention(q, k, v, self.state, None, tree_parents(parents, q), per_sequence(lengths, q, "lengths", 0, q.shape[2]),
                                      self.inv_temperature, self.a0, self.a1, self.a2, self.p, out)
 
     def accept(self, k, v, last, parents=None):
         """Takes drafted tokens into the state: the path from the root to node last[i] for every sequence i, nothing where last[i] is
-        -1.  k, v, parents as `verify` had them; last: int32 (b,).  tokens_seen counts the longest path that the drafts can have."""
+        -1.  k, v, parents as `verify` had them; last: int32 (b,).  Can be captured with last and parents on the device.  tokens_seen, one number
+        for all sequences, grows by the longest path that the drafts can have: from then on it is a bound, not a length."""
         _ext().tree_accept(k, v, self.state, per_sequence(last, k, "last", -1, k.shape[2] - 1), None, tree_parents(parents, k), self.p)
         self.tokens_seen += k.shape[2]
 
@@ -111,8 +112,9 @@ def _is_there(x):
 
 
 def per_sequence(x, like, name, low, high):
-    """One number per sequence as an int32 tensor beside `like`.  What lies on the host is checked to be in low .. high; what lies on the
-    device is not read here (the kernels treat other numbers as their documentation says), and int32 there goes on as it is."""
+    """One number per sequence as an int32 tensor beside `like`.  What lies on the host is checked to be in low .. high and copied, for which
+    the call waits and which cannot be captured; what lies on the device is not read here (the kernels treat other numbers as their
+    documentation says), and int32 there goes on as it is."""
     if _is_there(x):
         return x
     x = _whole(x, name)
@@ -145,4 +147,12 @@ def _whole(x, name):
 def _int32(x, like, low, high):
     if x.is_cuda:   # what is out of range stays so when it loses its upper bits
         x = x.clamp(low - 1, high + 1)
+    else:
+        refuse_capture(like.device)
     return x.to(device=like.device, dtype=torch.int32)
+
+
+def refuse_capture(device):
+    """For what copies from the host and waits for it: said before the copy, so that the capture goes on without the call."""
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("numbers on the host cannot go into a CUDA graph: pass int32 tensors on the device")

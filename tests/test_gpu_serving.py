@@ -717,6 +717,33 @@ def test_serving_calls_replay_from_graphs():
     assert torch.equal(eager[0].table, captured[0].table) and torch.equal(eager[0].state, captured[0].state) and torch.equal(eager[4], captured[4])
 
 
+def test_numbers_on_the_host_are_refused_during_a_capture():
+    """The refusal comes before the copy: the capture goes on without the call, and the cache stays as it was."""
+    from reproducing_fastmax_results_b200 import FastmaxCache
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    cache = FastmaxCache(3, 2, 16, temperature=10.0)
+    assert cache.begin([0, 1, 2]).item() == 0
+    cache.state[:, 0] = states(3, 2, 16, 2, gen)
+    x = [torch.randn(3, 2, 4, 16, device="cuda", generator=gen) for _ in range(3)]
+    parents, lengths, last = [[-1, 0, 0, 1]] * 3, [4, 2, 0], [3, -1, 0]
+    ref = cache.verify(*x, parents=parents, lengths=lengths)
+    before, table = cache.state.clone(), cache.table.clone()
+    on_device = i32(parents), i32(lengths), i32(last)
+    out = torch.zeros_like(x[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.begin([1]), lambda: cache.end([0]), lambda: cache.arrange([0, 0, 1]), lambda: cache.verify(*x, parents=parents),
+                     lambda: cache.verify(*x, lengths=torch.tensor(lengths)), lambda: cache.accept(x[1], x[2], last), lambda: cache.prefill(*x, [0, 1, 2])):
+            with pytest.raises(RuntimeError, match="graph"):
+                call()
+        cache.verify(*x, parents=on_device[0], lengths=on_device[1], out=out)
+    assert torch.equal(cache.state, before) and torch.equal(cache.table, table)
+    graph.replay()
+    assert torch.equal(out, ref) and torch.equal(cache.state, before)
+
+
 def test_calls_on_two_streams_keep_apart():
     from reproducing_fastmax_results_b200 import FastmaxCache
 
