@@ -97,7 +97,6 @@ class PagesCopyArgs(C.Structure):
                 ("count", C.c_int32), ("reserved", C.c_int32)]
 
 
-TREE_NODES = 64   # FASTMAX_TREE_NODES
 CACHE_PAGES = 32768   # FASTMAX_CACHE_PAGES
 
 

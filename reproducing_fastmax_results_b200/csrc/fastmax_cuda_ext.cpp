@@ -748,7 +748,6 @@ PYBIND11_MODULE(fastmax_cuda, m) {
   m.def("cache_compact", &cache_compact, "live pages move to the front: returns their number", release());
   m.def("pages_copy", &pages_copy, "pages of src by src_index into pages of dst by dst_index", py::arg("src"), py::arg("dst"), py::arg("src_index"),
         py::arg("dst_index"), py::arg("count"), release());
-  m.attr("TREE_NODES") = (int)FASTMAX_TREE_NODES;
   m.def("normalize_forward", &normalize_forward, "q/k normalisation: returns [y, stats]", release());
   m.def("normalize_backward", &normalize_backward, "gradient of the q/k normalisation", release());
   m.def("key_prologue", &key_prologue, "k <- k * inv_temp + rpe rows, in place", py::arg("k"), py::arg("inv_temp"),

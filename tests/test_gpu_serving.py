@@ -337,6 +337,53 @@ def test_steps_of_many_heads_on_pages(batch, heads, d, order, dtype):
     assert torch.equal(o2, o) and torch.equal(again, cache)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,heads,d,order", [(3, 2, 64, 2), (9, 16, 64, 2), (17, 8, 32, 2), (12, 13, 64, 1), (70, 16, 16, 2)])   # few heads, many
+def test_a_step_without_a_table(batch, heads, d, order, dtype):
+    """No table: sequence i has page i, and the pages behind the last sequence stay as they were.  The same bits as with that table."""
+    from reproducing_fastmax_results_b200 import _lib as L
+
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    cache = states(batch + 2, heads, d, order, gen, layers=2)
+    before, tabled = cache.clone(), cache.clone()
+    q, k, v = (torch.randn(batch, heads, d, device="cuda", generator=gen).to(dtype) for _ in range(3))
+    o, g = L.decode_step_paged(q, k, v, cache[:, 1], None, 0.1, *A, order)
+    ref, gref = L.decode_step_paged(q, k, v, tabled[:, 1], i32(range(batch)), 0.1, *A, order)
+    assert torch.equal(o, ref) and torch.equal(g, gref) and torch.equal(cache, tabled)
+    assert torch.equal(cache[:, 0], before[:, 0]) and torch.equal(cache[batch:], before[batch:])
+    for i in (0, batch - 1):
+        j = heads - 1
+        old, kk, vv = host(before[i, 1, j]), host(k[i, j])[None], host(v[i, j])[None]
+        oref, _, size, _ = so.tree(host(q[i, j])[None], kk, vv, old, [-1], order, A, 0.1)
+        rounding = 2.0 ** (-8 if dtype == torch.bfloat16 else -24)
+        assert (np.abs(host(o[i, j])[None] - oref) <= rounding * np.abs(oref) + so.SUMS_F32 * size).all()
+
+
+@pytest.mark.parametrize("heads", [2, 48])   # one launch, two
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_step_may_write_into_its_inputs(which, heads):
+    """The output in the place of q, k or v, views of one projection: what it gives elsewhere."""
+    from reproducing_fastmax_results_b200 import FastmaxCache
+
+    gen = torch.Generator(device="cuda").manual_seed(heads)
+    qkv = torch.randn(6, 3, heads, 1, 64, device="cuda", generator=gen).bfloat16()
+    start = states(6, heads, 64, 2, gen)
+    results = []
+    for place in (False, True):
+        cache = FastmaxCache(6, heads, 64, temperature=10.0)
+        assert cache.begin(range(5)).item() == 0
+        cache.state[:, 0] = start
+        x = qkv.clone()
+        out = x[:, which] if place else qkv[:, which].clone()   # the absent place's rows stay as they are
+        for _ in range(2):
+            x.copy_(qkv)
+            o = cache.step(x[:, 0], x[:, 1], x[:, 2], out=out)
+            others = [i for i in range(3) if i != which]
+            assert torch.equal(x[:, others], qkv[:, others]) and torch.equal(x[5], qkv[5])
+        results.append((o.clone(), cache.state.clone()))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
 # ---- pages -----------------------------------------------------------------------------------------------------------------
 def arrange_and_compare(table, sources, pages, floats, seed):
     from reproducing_fastmax_results_b200.attention import _ext
