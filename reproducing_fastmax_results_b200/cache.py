@@ -94,7 +94,7 @@ class FastmaxCache:
         if continues:
             before = torch.zeros((len(places), *states.shape[1:]), dtype=torch.float32, device=states.device)
             _ext().pages_copy(states, before, index, None, len(places))
-        with torch.cuda.device(states.device):
+        with torch.cuda.device(states.device.index):
             o, _, after = _lib.forward(q, k, v, True, self.inv_temperature, self.a0, self.a1, self.a2, self.p, state_in=before, want_state=True,
                                        flags=_lib.FLAG_PAIRWISE)
         _ext().pages_copy(after, states, None, index, len(places))

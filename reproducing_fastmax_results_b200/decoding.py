@@ -56,7 +56,7 @@ class FastmaxDecoder:
         """Causal attention of a (b, h, n, d) block that continues the sequence seen so far.  Returns o (b, h, n, d)
         and adds the block's keys and values to the state."""
         check_prompts(q, k, v, self.batch, self.state)
-        with torch.cuda.device(self.state.device):
+        with torch.cuda.device(self.state.device.index):
             o, _, state = _lib.forward(q, k, v, True, self.inv_temperature, self.a0, self.a1, self.a2, self.p,
                                        state_in=self.state if self.tokens_seen else None, want_state=True,
                                        flags=_lib.FLAG_PAIRWISE)
@@ -92,19 +92,19 @@ class FastmaxDecoder:
 def check_prompts(q, k, v, batch, state):
     """Prompts' q, k, v for the `batch` sequences of `state` (float32 (..., heads, rows, d + 4)): all of it is refused here, before anything is
     launched, since the binding that prompts go through takes the sizes, the type and the device of all three from q."""
-    heads, d = state.shape[-3], state.shape[-1] - 4
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4 or tuple(t.shape) != (batch, heads, q.shape[2], d):
-            raise ValueError(f"{name}: expected ({batch}, {heads}, n, {d}), got {tuple(t.shape)}")
-    if q.shape[2] == 0:
+    shape, sizes = q.shape, state.shape
+    if len(shape) != 4 or k.shape != shape or v.shape != shape or shape[0] != batch or shape[1] != sizes[-3] or shape[3] != sizes[-1] - 4:
+        raise ValueError(f"q, k, v: expected ({batch}, {sizes[-3]}, n, {sizes[-1] - 4}), got {tuple(shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if shape[2] == 0:
         raise ValueError("a prompt needs a token")
+    dtype, device = q.dtype, state.device
     _lib.dtype_code(q)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise RuntimeError(f"dtypes differ: q {q.dtype}, k {k.dtype}, v {v.dtype}")
-    if any(t.stride(3) != 1 for t in (q, k, v)):
+    if k.dtype != dtype or v.dtype != dtype:
+        raise RuntimeError(f"dtypes differ: q {dtype}, k {k.dtype}, v {v.dtype}")
+    if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1:
         raise RuntimeError("the head dim must be contiguous")
-    if any(not t.is_cuda or t.device != state.device for t in (q, k, v)):
-        raise RuntimeError(f"q, k, v must be CUDA tensors on the state's device {state.device}, got {q.device}, {k.device}, {v.device}")
+    if device.type != "cuda" or q.device != device or k.device != device or v.device != device:
+        raise RuntimeError(f"q, k, v must be CUDA tensors on the state's device {device}, got {q.device}, {k.device}, {v.device}")
 
 
 def _is_there(x):
