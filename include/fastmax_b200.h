@@ -232,7 +232,10 @@ int32_t fastmax_decode_step_paged(const fastmax_problem* pb, const fastmax_paged
  *       Rows behind it, and all rows of absent sequences, are not written.
  *   q, k, v: all nq rows of every sequence must be readable, whatever table and lengths say: they are asked for before it is known which
  *       of them count.  What stands in rows that do not count changes nothing.
- *   o must not share memory with q, k, v or the state. */
+ *   o must not share memory with q, k, v or the state.
+ *   Precision: float32 tensors keep 24 bits of every term; with bfloat16 tensors the state enters with 16 bits (two bfloat16 pieces), in o
+ *       and in g alike, where fastmax_decode_step has 24.  An infinity in q, k or the state may come out as NaN where the sum would be infinite (the pieces
+ *       behind it are inf - inf).  What is not finite in q reaches its own node, in k or v the nodes that see it. */
 #define FASTMAX_TREE_NODES 64
 typedef struct {
   fastmax_tensor q, k, v;

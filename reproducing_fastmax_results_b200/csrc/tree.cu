@@ -206,12 +206,13 @@ __device__ __forceinline__ float* head_state(const TreeParams& P, int b, int h, 
 // by the copy engine into a ring of slots; whichever warp is done last with a step asks for the units that take its place.
 //
 // Products by warps and not tcgen05: the operand that streams is the state, which has to be split on its way.  In registers it goes straight from
-// one wide load into the product; for tcgen05 its pieces would have to be written to shared memory once more, the 64 columns of a state
-// would fill half of the 128 rows, and x_m would have to be applied to tensor memory 64 times a head.
+// one wide load into the product; for tcgen05 its pieces would have to be written to shared memory once more.  Up to 8 nodes that could only
+// lose (HBM bounds it); for the largest trees, where the accumulators of this form leave room for 16 warps an SM, it has not been built or measured.
 //
 // What bounds it (bf16, 512 heads of 64 dims, order 2, 330 MB of states, 50 us at the copy rate): up to 8 nodes HBM, 53.9 us; 25 nodes 70 us and 64
 // nodes 116 us, the chain of a step (load, split, product, scale: issue slots 51 and 47 %, tensor pipe active 34 and 41 %) and the rounds of blocks:
-// 288 heads of 25 nodes take 37 us, 464 70 us, 592 72 us.  Built and left: 25 nodes, 464 heads (70 us): sixteen warps a block and one block to an SM
+// 288 heads of 25 nodes take 38 us, 464 70 us, 592 73 us.  float32 (512 heads, 64 dims; six products where bfloat16 has two): 8 nodes 65 us, 16 81, 25 132,
+// 40 211, 64 276.  Built and left (bf16): 25 nodes, 464 heads (70 us): sixteen warps a block and one block to an SM
 // 94, two of them 91, four warps 78, three blocks of eight 90; slots 3 / 4 / 5: 85 / 71 / 70; halves of heads in clusters 79.  Copies by the
 // threads instead of the copy engine: 91 instead of 71 us for 8 nodes at that stage.  The tree's sums as products, too: chains of 64 nodes 115
 // instead of 134 us, but trees as before and small ones 1 to 3 % slower.  The last units of rows of odd length paired up with m and n exchanged (18
@@ -290,7 +291,9 @@ struct TreeGeo {
   static constexpr int CG = D / 16;                    // groups of 16 columns of the state: one to a warp
   // Blocks to an SM, and warps that share a group of columns and divide the rows m of a unit among them: eight warps for 64 dims, four for fewer (us
   // with eight warps, two blocks / four warps, four blocks, 512 heads: 32 dims, 8 nodes 16.2 / 11.6, 25 nodes 21.6 / 16.9; 16 dims, 16 nodes 11.6 / 7.5).
-  static constexpr bool LARGE = NT == 8 && sizeof(T) == 4;   // registers for half as many
+  // float32 trees of more than 32 nodes: half as many blocks, so that 32 and 16 dims have 255 and 238 registers a thread; 64 dims have one block of
+  // sixteen warps with 128 and keep 492 bytes of them in local memory (512 heads of 64 nodes: 276 us).
+  static constexpr bool LARGE = NT == 8 && sizeof(T) == 4;
   static constexpr int BLOCKS = (D == 64 ? 2 : 4) / (LARGE ? 2 : 1);
   static constexpr int KG = D == 16 || (D == 64 && LARGE) ? 4 : 2;
   static constexpr int RI = 8 / KG;
@@ -829,7 +832,11 @@ static cudaError_t launch_attention(const TreeParams& P, int bh, cudaStream_t st
   using G = TreeGeo<T, D, NT>;
   cudaError_t e = allow_bytes<attention_kernel<T, D, NT>>(G::BYTES);
   if (e != cudaSuccess) return e;
-  // A head is divided among blocks of a cluster as far as there are then no more than two of them for every SM, each with two units or more.
+  // A head is divided among blocks of a cluster as far as there are then no more than two of them for every SM, each with two units or more.  us
+  // with 1 / 2 / 4 blocks a head, order 2, float32 heads of 32 dims, 5 nodes: 37 heads 9.5 / 7.8 / 6.8, 74 heads 9.4 / 8.0 / 7.9, 148 heads 9.9 / 9.3 /
+  // 14.3, 288 heads 10.9 / 10.7 / 20.5, 400 heads 13.9 / 19.0 / 23.3; bf16, 25 nodes: 37 heads 10.7 / 8.9 / 8.4, 148 heads 11.2 / 10.6 / 17.9, 288
+  // heads 13.1 / 13.7 / 26.5, so a third or fourth block to an SM gains nothing although there is room for them.  16 dims, 1 / 2 blocks (of two
+  // units): 8 nodes, 8 heads 4.9 / 5.6, 148 heads 5.0 / 5.7; float32, 25 nodes, 8 heads 7.5 / 7.6, 148 heads 7.8 / 8.7.
   const int units = (P.order == 2 ? Geo<D>::NPAIRS : 0) + 1;
   int cl = 1;
   while (cl < 8 && 2LL * cl * bh <= (G::BLOCKS < 2 ? 1LL : 2LL) * sm_count() && 4 * cl <= units + 1) cl *= 2;
