@@ -266,8 +266,8 @@ def _attach_key_moments(lib, pb, args, key_moments, device):
 
 
 def forward(q, k, v, causal, inv_temp, a0=1.0, a1=1.0, a2=0.5, order=2, state_in=None, want_state=False,
-            want_output=True, flags=0, out=None, key_moments=None):
-    """Calls fastmax_forward on (b,h,n,d) CUDA tensors.  Returns (o, g, state_out).  `out`: optional (b,h,n,d) tensor
+            want_output=True, flags=0, out=None, key_moments=None, state_out=None):
+    """Calls fastmax_forward on (b,h,n,d) CUDA tensors.  Returns (o, g, state_out), which with want_state is `state_out` or a new tensor.  `out`: optional (b,h,n,d) tensor
     of any strides (unit stride on d) that receives o, e.g. the transposed view of a (b, n, h*d) buffer.
     `key_moments`: optional KeyMoments holder for this (k, v)."""
     import torch
@@ -286,8 +286,9 @@ def forward(q, k, v, causal, inv_temp, a0=1.0, a1=1.0, a2=0.5, order=2, state_in
         assert state_in.is_contiguous() and state_in.dtype == torch.float32
         args.state_in = state_in.data_ptr()
     if want_state:
-        sout = torch.empty((q.shape[0], q.shape[1], lib.fastmax_state_rows(pb.d, pb.order), lib.fastmax_state_ld(pb.d)),
-                           dtype=torch.float32, device=q.device)
+        shape = (q.shape[0], q.shape[1], lib.fastmax_state_rows(pb.d, pb.order), lib.fastmax_state_ld(pb.d))
+        sout = torch.empty(shape, dtype=torch.float32, device=q.device) if state_out is None else state_out
+        assert sout.shape == shape and sout.dtype == torch.float32 and sout.is_contiguous()
         args.state_out = sout.data_ptr()
     if key_moments is not None:
         _attach_key_moments(lib, pb, args, key_moments, q.device)

@@ -29,7 +29,7 @@ class FastmaxDecoder:
     batch, heads, d, p: problem geometry (d in {16, 32, 64}; p = polynomial order 1 or 2).
     temperature, a0, a1, a2: as in `fastmax_custom` (scores are q.k / temperature).
     The state is float32 (batch, heads, rows, d + 4) in the layout of `fastmax_forward`'s state_out and is
-    updated in place by every call.
+    updated in place by every call, so a step that was captured into a CUDA graph goes on from whatever was read last.
     """
 
     def __init__(self, batch, heads, d, p=2, temperature=1.0, a0=1.0, a1=1.0, a2=0.5, device="cuda"):
@@ -57,10 +57,12 @@ class FastmaxDecoder:
         and adds the block's keys and values to the state."""
         check_prompts(q, k, v, self.batch, self.state)
         with torch.cuda.device(self.state.device.index):
-            o, _, state = _lib.forward(q, k, v, True, self.inv_temperature, self.a0, self.a1, self.a2, self.p,
-                                       state_in=self.state if self.tokens_seen else None, want_state=True,
-                                       flags=_lib.FLAG_PAIRWISE)
-        self.state = state
+            before = self.state if self.tokens_seen else None
+            # the state keeps its memory, which a captured step reads; the call does not take one array as both of its states
+            o, _, state = _lib.forward(q, k, v, True, self.inv_temperature, self.a0, self.a1, self.a2, self.p, state_in=before,
+                                       want_state=True, flags=_lib.FLAG_PAIRWISE, state_out=None if self.tokens_seen else self.state)
+            if before is not None:
+                self.state.copy_(state)
         self.tokens_seen += q.shape[2]
         return o
 

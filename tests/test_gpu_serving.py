@@ -764,6 +764,47 @@ def test_serving_calls_replay_from_graphs():
     assert torch.equal(eager[0].table, captured[0].table) and torch.equal(eager[0].state, captured[0].state) and torch.equal(eager[4], captured[4])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_calls_of_a_decoder_serve_the_next_prompt(dtype):
+    """The state keeps its memory: a step, a tree and its path, captured once, go on from whatever prompt was read last."""
+    from reproducing_fastmax_results_b200 import FastmaxDecoder
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    prompts = [[torch.randn(2, 3, n, 64, device="cuda", generator=gen).to(dtype) for _ in range(3)] for n in (9, 30, 4)]
+    x = [torch.randn(2, 3, 5, 64, device="cuda", generator=gen).to(dtype) for _ in range(3)]
+    last = i32([3, -1])
+
+    def serve(dec, tree, token):
+        dec.verify(*x, out=tree)
+        dec.accept(x[1], x[2], last)
+        dec.step(*(t[:, :, 0] for t in x), out=token)
+
+    def read(dec, which):
+        dec.reset()
+        dec.prefill(*prompts[which])
+        if which == 1:
+            dec.prefill(*prompts[2])   # goes on
+
+    eager, captured = FastmaxDecoder(2, 3, 64, temperature=10.0), FastmaxDecoder(2, 3, 64, temperature=10.0)
+    outs = [[torch.zeros_like(x[0]), torch.zeros_like(x[0][:, :, 0])] for _ in range(2)]
+    read(eager, 0)
+    serve(eager, *outs[0])
+    memory = captured.state.data_ptr()
+    read(captured, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        serve(captured, *outs[1])
+    for which in (0, 1, 2):
+        read(eager, which)
+        serve(eager, *outs[0])
+        read(captured, which)
+        assert captured.state.data_ptr() == memory
+        graph.replay()
+        assert torch.equal(eager.state, captured.state)
+        assert all(torch.equal(a, b) and float(a.float().abs().sum()) > 0 for a, b in zip(*outs))
+
+
 def test_numbers_on_the_host_are_refused_during_a_capture():
     """The refusal comes before the copy: the capture goes on without the call, and the cache stays as it was."""
     from reproducing_fastmax_results_b200 import FastmaxCache
