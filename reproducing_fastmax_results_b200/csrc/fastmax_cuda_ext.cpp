@@ -188,6 +188,17 @@ fastmax_problem make_problem(const torch::Tensor& q, const torch::Tensor& k, boo
   return pb;
 }
 
+// The kernels take the batch, the heads, the head dim, the type and the device from q, and the number of tokens from k.
+void check_qkv(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k, v must be (b, h, n, d)");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3) && v.sizes() == k.sizes(),
+              "q, k, v: one batch, number of heads and head dim, and as many values as keys expected, got ", q.sizes(), ", ", k.sizes(), " and ",
+              v.sizes());
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k, v dtypes differ");
+  CHECK_CUDA(q); CHECK_CUDA(k); CHECK_CUDA(v);
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "q, k, v must be on one device");
+}
+
 // returns (o, g, state_out or empty); with key_moments given or want_key_moments set a fourth entry follows: the
 // per-segment key moments this call read or wrote (undefined when the call has none), to be handed to the next call
 // with the same k and v (fastmax_forward_args.key_moments_in / _out)
@@ -195,9 +206,7 @@ std::vector<torch::Tensor> forward(torch::Tensor q, torch::Tensor k, torch::Tens
                                    double a0, double a1, double a2, int64_t p, c10::optional<torch::Tensor> state_in,
                                    bool want_state, bool want_output, int64_t flags, c10::optional<torch::Tensor> out,
                                    c10::optional<torch::Tensor> key_moments, bool want_key_moments) {
-  CHECK_CUDA(q); CHECK_CUDA(k); CHECK_CUDA(v);
-  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k, v must be (b, h, n, d)");
-  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k, v dtypes differ");
+  check_qkv(q, k, v);
   const c10::cuda::CUDAGuard guard(q.device());
   auto stream = at::cuda::getCurrentCUDAStream().stream();
   fastmax_problem pb = make_problem(q, k, causal, inv_temp, a0, a1, a2, p, flags);
@@ -446,6 +455,7 @@ struct FastmaxNode : public torch::autograd::Function<FastmaxNode> {
       q = readable(q); k = readable(k); v = readable(v);
     }
     if (normalize) {
+      check_qkv(q, k, v);
       auto n = normalize_forward_qk(q, k, lim);
       q = n[0]; stats_q = n[1];
       k = n[2]; stats_k = n[3];

@@ -254,6 +254,21 @@ def test_outputs_whose_rows_lie_on_one_another_are_refused():
                 serve.step(x[:, :, 0], x[:, :, 0], x[:, :, 0], out=out.expand(3, 2, 16))
 
 
+def test_the_operator_refuses_sizes_that_do_not_fit_before_any_launch():
+    """A v shorter than k, or keys of fewer heads than queries, would be read past their end."""
+    from reproducing_fastmax_results_b200 import fastmax_custom
+
+    x = torch.zeros(2, 3, 8, 16)
+    for k, v in ((x, x[:, :, :7]), (x[:, :, :7], x), (x[:1], x[:1]), (x[:, :2], x[:, :2]), (x, x[:, :1]), (x[..., :8], x[..., :8])):
+        for normalize in (False, True):
+            with pytest.raises(RuntimeError, match="as many values as keys"):
+                fastmax_custom(x, k, v, None, None, True, 0.0, normalize)
+    with pytest.raises(RuntimeError, match="dtypes differ"):
+        fastmax_custom(x, x.bfloat16(), x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fastmax_custom(x, x[:, :, :5], x[:, :, :5])
+
+
 # ---- the oracle ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("order", [1, 2])
 @pytest.mark.parametrize("d", [16, 32])
